@@ -10,6 +10,16 @@ reference's pybind module, src/main.cpp:1594-1602, plus the 2-D forms):
                                        batched GEMM on NCHW (no layout copies)
     attention(query, key, value, scale=None)
                                        softmax(scale * Q K^T) V on [B, H, S, D]
+    attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k=None,
+                     causal=True, scale=None, out=None)
+                                       the same for packed sequences [tokens, heads, D]
+                                       with grouped heads and a causal mask
+    attention_paged(query, key_cache, value_cache, page_table, seqlens_k, ...)
+                                       new tokens over a paged key / value cache
+    kv_cache_write(key, value, key_cache, value_cache, slots, ...) /
+    kv_cache_read(key_cache, value_cache, slots, ...)
+                                       tokens into / out of the cache (fp16, bf16, fp32,
+                                       or e4m3 with a power-of-two scale a vector)
     fp16_matmul(a, b) / bf16_matmul(a, b) / fp32_matmul(a, b)
                                        a[M,K] @ b[K,N] -> [M,N]
 
@@ -26,7 +36,8 @@ import torch  # noqa: F401  (loads libtorch / c10 before the shim)
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcmpx.so")
 
-_OPS = ("linear", "bmm", "conv2d", "attention", "fp16_matmul", "bf16_matmul", "fp32_matmul", "_set_path", "_matmul_into", "_matmul_gather_ce", "version")
+_OPS = ("linear", "bmm", "conv2d", "attention", "attention_varlen", "attention_paged", "kv_cache_write",
+        "kv_cache_read", "fp16_matmul", "bf16_matmul", "fp32_matmul", "_set_path", "_matmul_into", "_matmul_gather_ce", "version")
 
 
 def _load_ext():
@@ -52,4 +63,5 @@ def __getattr__(name):
     raise AttributeError(f"module 'cmp_ext_b200' has no attribute {name!r}")
 
 
-__all__ = ["linear", "bmm", "conv2d", "attention", "fp16_matmul", "bf16_matmul", "fp32_matmul", "LIB_PATH", "version"]
+__all__ = ["linear", "bmm", "conv2d", "attention", "attention_varlen", "attention_paged", "kv_cache_write",
+           "kv_cache_read", "fp16_matmul", "bf16_matmul", "fp32_matmul", "LIB_PATH", "version"]

@@ -41,13 +41,12 @@
 #include <cstdio>
 #include <cstdlib>
 
+#include "attention_math.cuh"
 #include "internal.h"
 #include "ptx.cuh"
 
 namespace cmpx {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int TPR>
 struct AttnCfg {
@@ -73,59 +72,6 @@ struct AttnParams {
 __device__ __forceinline__ void rec_err(int* err, volatile int* abort, int code) {
   *abort = 1;
   atomicCAS(err, 0, code);
-}
-
-// 2^x with the hardware's approximate base-2 exponential (ex2.approx,
-// relative error ~2^-22; results below 2^-126 flush to zero, which a softmax
-// weight that small does not need).  2^-inf = 0.
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Blackwell's paired fp32 arithmetic: two lanes in one 64-bit register, one
-// instruction, each lane rounded exactly as the scalar fmaf / + (.rn), so a
-// softmax written with them gives the same bits as the scalar one with about
-// half the issue slots.  max3f is the three-input maximum (exact).
-__device__ __forceinline__ uint64_t f2pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 f2unpack(uint64_t r) {
-  float2 v;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-  return v;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half*) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
 }
 
 // PK = 1: the softmax uses the paired / three-input instructions above (same
@@ -898,22 +844,8 @@ __global__ void __launch_bounds__(PPCfg<D>::THREADS, 1)
 }
 
 // ------------------------------------------------------------------ CUDA cores
-template <typename T>
-__device__ __forceinline__ float ldf(const T* p);
-template <>
-__device__ __forceinline__ float ldf<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float ldf<__half>(const __half* p) { return __half2float(*p); }
-template <>
-__device__ __forceinline__ float ldf<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void stf(float* p, float v) { *p = v; }
-__device__ __forceinline__ void stf(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void stf(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
 // One warp per query row; lane d holds output columns d, d+32, ... (up to
 // kSimtMaxD / 32 of them).  Online softmax in fp32 over all S keys.
-constexpr int kSimtMaxD = 512;
-
 template <typename T>
 __global__ void __launch_bounds__(128) attention_simt_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                              const T* __restrict__ V, T* __restrict__ O,

@@ -1,0 +1,80 @@
+// Problem description shared by the kernels behind cmpx_attention_seq
+// (attention_seq.cu: checks, dispatch, CUDA-core kernel).
+#pragma once
+#include <cstdint>
+
+#include "internal.h"
+
+namespace cmpx {
+
+// Keys or values: rows of one kv head, in a packed tensor or in pages.
+struct SeqKV {
+  const void* base;
+  int64_t row, head, page;        // strides (elements)
+  const uint8_t* scale;           // e8m0 bytes of an 8-bit cache, else nullptr
+  int64_t s_row, s_head, s_page;  // their strides
+};
+
+struct SeqProblem {
+  const void* Q;
+  void* O;
+  int64_t q_token, q_head, o_token, o_head;  // strides (elements)
+  SeqKV k, v;
+  const int* cu_q;    // nullptr: uniform_n tokens each
+  const int* cu_k;    // packed form
+  const int* table;   // paged form, else nullptr
+  const int* lens_k;  // paged form
+  int64_t table_stride;
+  int batch, uniform_n, tokens_q, tokens_kv, heads_q, heads_kv, group, d;
+  int page_size, pages, max_keys;  // max_keys: keys a row of the page table can name
+  float scale_log2;                // scale * log2 e
+  int causal, zero_rest;
+};
+
+// One sequence: query tokens [q0, q0 + n), keys [k0, k0 + len) of the packed
+// tensor (k0 = 0 in the paged form).
+struct Seq {
+  int q0, n, k0, len;
+};
+
+#ifdef __CUDACC__
+// Clamped, so that lengths no caller should pass never lead outside a tensor.
+__device__ __forceinline__ int2 seq_queries(const SeqProblem& p, int b) {
+  if (p.cu_q == nullptr) return make_int2(b * p.uniform_n, p.uniform_n);
+  const int q0 = min(max(__ldg(p.cu_q + b), 0), p.tokens_q);
+  const int q1 = min(max(__ldg(p.cu_q + b + 1), q0), p.tokens_q);
+  return make_int2(q0, q1 - q0);
+}
+__device__ __forceinline__ Seq seq_of(const SeqProblem& p, int b) {
+  Seq s;
+  const int2 q = seq_queries(p, b);
+  s.q0 = q.x;
+  s.n = q.y;
+  if (p.table != nullptr) {
+    s.k0 = 0;
+    s.len = min(max(__ldg(p.lens_k + b), 0), p.max_keys);
+  } else if (p.cu_k != nullptr) {
+    s.k0 = min(max(__ldg(p.cu_k + b), 0), p.tokens_kv);
+    s.len = min(max(__ldg(p.cu_k + b + 1), s.k0), p.tokens_kv) - s.k0;
+  } else {
+    s.k0 = min(s.q0, p.tokens_kv);
+    s.len = min(s.n, p.tokens_kv - s.k0);
+  }
+  return s;
+}
+// Keys that query token i of a sequence sees: the first seq_limit() of them.
+__device__ __forceinline__ int seq_limit(const SeqProblem& p, const Seq& s, int i) {
+  return p.causal ? min(max(s.len - s.n + i + 1, 0), s.len) : s.len;
+}
+// First token that no sequence holds any more (cu_seqlens_q[batch], clamped),
+// and the number of tokens before the first sequence.
+__device__ __forceinline__ int2 seq_rest(const SeqProblem& p) {
+  if (p.cu_q == nullptr) return make_int2(0, p.batch * p.uniform_n);
+  return make_int2(min(max(__ldg(p.cu_q), 0), p.tokens_q), min(max(__ldg(p.cu_q + p.batch), 0), p.tokens_q));
+}
+#endif
+
+// Host side of the kernels.  Each returns a cudaError_t of its launches.
+cudaError_t launch_seq_simt(const SeqProblem& p, int dtype, int kv_dtype, cudaStream_t s);
+
+}  // namespace cmpx

@@ -20,8 +20,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "cmpx.h"
@@ -418,6 +421,390 @@ torch::Tensor attention(torch::Tensor query, torch::Tensor key, torch::Tensor va
   return out;
 }
 
+// ------------------------------------------------- packed sequences, paged cache
+// Everything below checks shapes, types and devices on the host and leaves
+// lengths, page numbers and slots, which live on the device, to the kernels
+// (they clamp or skip what is out of range).
+
+// The bytes a strided tensor spans, for overlap checks.
+std::pair<const char*, const char*> span_of(const torch::Tensor& t) {
+  const char* p = static_cast<const char*>(t.data_ptr());
+  if (t.numel() == 0) return {p, p};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {p, p + (last + 1) * t.element_size()};
+}
+bool overlaps(const torch::Tensor& a, const torch::Tensor& b) {
+  const auto x = span_of(a), y = span_of(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+// A tensor that a kernel writes in place: unit stride along D, and no two
+// elements on one address.
+void check_writable(const torch::Tensor& t, const char* name, bool unit_last) {
+  if (t.numel() == 0) return;
+  TORCH_CHECK(!unit_last || t.stride(-1) == 1 || t.size(-1) == 1, name, " must be contiguous along its last dimension");
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+  std::sort(dims.begin(), dims.end());
+  int64_t reach = 1;  // elements the dimensions so far span
+  for (const auto& d : dims) {
+    TORCH_CHECK(d.first >= reach, name, " must not overlap itself");
+    reach += (d.second - 1) * d.first;
+  }
+}
+
+// query / key / value as the kernels take them: unit stride along D, and for
+// 16-bit types strides and addresses on 16 bytes (a copy otherwise).
+torch::Tensor rows16(torch::Tensor t) {
+  if (t.numel() == 0) return t;
+  const int64_t es = t.element_size();
+  bool ok = t.stride(-1) == 1 || t.size(-1) == 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) == 1 || t.stride(i) * es % 16 == 0);
+  ok = ok && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Stride of a dimension; one of a single element never moves, so it counts as
+// `packed`, whatever the tensor says.
+int64_t stride_or(const torch::Tensor& t, int64_t dim, int64_t packed) {
+  return t.size(dim) > 1 ? t.stride(dim) : packed;
+}
+
+torch::Tensor index_arg(const torch::Tensor& t, const char* name, int64_t size, const torch::Tensor& like) {
+  TORCH_CHECK(t.dim() == 1, name, " must be 1D");
+  TORCH_CHECK(t.size(0) == size, name, " must have ", size, " elements, got ", t.size(0));
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32");
+  TORCH_CHECK(t.device() == like.device(), "Device mismatch");
+  return t;
+}
+
+torch::Tensor seq_output(const c10::optional<torch::Tensor>& out, const torch::Tensor& query,
+                         const std::vector<torch::Tensor>& inputs) {
+  if (!out.has_value() || !out->defined()) return torch::empty(query.sizes(), query.options());
+  TORCH_CHECK(out->sizes() == query.sizes(), "out must have the query's shape");
+  TORCH_CHECK(out->scalar_type() == query.scalar_type(), "out must have the query's dtype");
+  TORCH_CHECK(out->device() == query.device(), "Device mismatch");
+  check_writable(*out, "out", true);
+  for (const auto& t : inputs)
+    if (t.defined()) TORCH_CHECK(!overlaps(*out, t), "out must not overlap an input");
+  return *out;
+}
+
+void set_query(cmpx_attention_seq_args& a, const torch::Tensor& q, const torch::Tensor& out) {
+  a.Q = q.data_ptr();
+  a.O = out.data_ptr();
+  a.tokens_q = q.size(0);
+  a.heads_q = q.size(1);
+  a.head_dim = q.size(2);
+  a.q_stride_token = stride_or(q, 0, q.size(1) * q.size(2));
+  a.q_stride_head = stride_or(q, 1, q.size(2));
+  a.o_stride_token = stride_or(out, 0, q.size(1) * q.size(2));
+  a.o_stride_head = stride_or(out, 1, q.size(2));
+}
+
+float seq_scale(const c10::optional<double>& scale, int64_t d) {
+  return scale.has_value() ? static_cast<float>(scale.value()) : 1.0f / std::sqrt(static_cast<float>(d));
+}
+
+void run_seq(cmpx_attention_seq_args& a, const torch::Tensor& q, const char* name) {
+  if (g_forced_path == CMPX_PATH_SIMT || g_forced_path == CMPX_PATH_TC || g_forced_path == CMPX_PATH_SKINNY)
+    a.path = g_forced_path;
+  torch::Tensor ws;
+  const size_t bytes = cmpx_attention_seq_workspace_size(&a);
+  if (bytes > 0) {
+    ws = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  check_status(cmpx_attention_seq(&a, current_stream()), name);
+}
+
+// softmax(scale * Q K^T) V for sequences packed along the token dimension:
+// query [Tq, Hq, D], key / value [Tk, Hkv, D], sequence b the tokens
+// [cu_seqlens[b], cu_seqlens[b + 1]).
+torch::Tensor attention_varlen(torch::Tensor query, torch::Tensor key, torch::Tensor value, torch::Tensor cu_seqlens_q,
+                               c10::optional<torch::Tensor> cu_seqlens_k, bool causal, c10::optional<double> scale,
+                               c10::optional<torch::Tensor> out_arg) {
+  TORCH_CHECK(query.dim() == 3, "Query must be 3D (Tokens, Heads, Dim)");
+  TORCH_CHECK(key.dim() == 3, "Key must be 3D");
+  TORCH_CHECK(value.dim() == 3, "Value must be 3D");
+  const int64_t D = query.size(2), Hkv = key.size(1);
+  TORCH_CHECK(key.size(2) == D, "Key shape mismatch");
+  TORCH_CHECK(value.sizes() == key.sizes(), "Value shape mismatch");
+  TORCH_CHECK(query.size(1) == 0 || (Hkv > 0 && query.size(1) % Hkv == 0),
+              "Query heads must be a multiple of key heads");
+  TORCH_CHECK(query.device() == key.device() && query.device() == value.device(), "Device mismatch");
+  TORCH_CHECK(key.scalar_type() == query.scalar_type() && value.scalar_type() == query.scalar_type(),
+              "Dtype mismatch");
+  const int dt = dtype_code(query.scalar_type());
+  TORCH_CHECK(dt >= 0, "Unsupported dtype for attention");
+  TORCH_CHECK(cu_seqlens_q.dim() == 1 && cu_seqlens_q.size(0) >= 1, "cu_seqlens_q must be 1D with batch + 1 elements");
+  const int64_t B = cu_seqlens_q.size(0) - 1;
+  torch::Tensor cu_q = index_arg(cu_seqlens_q, "cu_seqlens_q", B + 1, query);
+  torch::Tensor cu_k;
+  if (cu_seqlens_k.has_value() && cu_seqlens_k->defined())
+    cu_k = index_arg(*cu_seqlens_k, "cu_seqlens_k", B + 1, query);
+  else
+    TORCH_CHECK(key.size(0) == query.size(0), "Without cu_seqlens_k, key must have as many tokens as query");
+  TORCH_CHECK(query.is_cuda(), "attention_varlen expects CUDA tensors");
+  c10::cuda::CUDAGuard guard(query.device());
+  torch::Tensor out = seq_output(out_arg, query, {query, key, value, cu_seqlens_q, cu_k});
+  query = rows16(query);
+  key = rows16(key);
+  value = rows16(value);
+  cu_q = cu_q.contiguous();
+  if (cu_k.defined()) cu_k = cu_k.contiguous();
+  cmpx_attention_seq_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.dtype = a.kv_dtype = dt;
+  set_query(a, query, out);
+  a.K = key.data_ptr();
+  a.V = value.data_ptr();
+  a.batch = B;
+  a.heads_kv = Hkv;
+  a.tokens_kv = key.size(0);
+  a.k_stride_row = stride_or(key, 0, Hkv * D);
+  a.k_stride_head = stride_or(key, 1, D);
+  a.v_stride_row = stride_or(value, 0, Hkv * D);
+  a.v_stride_head = stride_or(value, 1, D);
+  a.cu_seqlens_q = cu_q.data_ptr<int>();
+  a.cu_seqlens_k = cu_k.defined() ? cu_k.data_ptr<int>() : nullptr;
+  a.scale = seq_scale(scale, D);
+  a.causal = causal;
+  a.zero_rest = !(out_arg.has_value() && out_arg->defined());
+  run_seq(a, query, "attention_varlen");
+  return out;
+}
+
+// Checks a paged cache's two tensors and (8-bit caches) their scales; returns
+// the cache's dtype code.
+int check_cache(const torch::Tensor& kc, const torch::Tensor& vc, const c10::optional<torch::Tensor>& ks,
+                const c10::optional<torch::Tensor>& vs, int64_t heads, int64_t D, const torch::Tensor& like) {
+  TORCH_CHECK(kc.dim() == 4, "key_cache must be 4D (Pages, Heads, Page size, Dim)");
+  TORCH_CHECK(vc.sizes() == kc.sizes(), "value_cache must have key_cache's shape");
+  TORCH_CHECK(heads < 0 || kc.size(1) == heads, "key_cache heads mismatch");
+  TORCH_CHECK(D < 0 || kc.size(3) == D, "key_cache head dim mismatch");
+  TORCH_CHECK(kc.size(2) > 0, "key_cache page size must be positive");
+  TORCH_CHECK(kc.device() == like.device() && vc.device() == like.device(), "Device mismatch");
+  TORCH_CHECK(vc.scalar_type() == kc.scalar_type(), "Dtype mismatch");
+  for (const auto* t : {&kc, &vc})
+    TORCH_CHECK(t->numel() == 0 || t->stride(3) == 1 || t->size(3) == 1,
+                "key_cache and value_cache must be contiguous along their last dimension");
+  const bool q8 = kc.scalar_type() == at::kFloat8_e4m3fn;
+  const bool given = ks.has_value() && ks->defined() && vs.has_value() && vs->defined();
+  if (!q8) {
+    TORCH_CHECK(!(ks.has_value() && ks->defined()) && !(vs.has_value() && vs->defined()),
+                "key_scale and value_scale belong to a float8_e4m3fn cache");
+    return dtype_code(kc.scalar_type());
+  }
+  TORCH_CHECK(given, "A float8_e4m3fn cache needs key_scale and value_scale");
+  for (const auto* t : {&*ks, &*vs}) {
+    TORCH_CHECK(t->scalar_type() == at::kFloat8_e8m0fnu, "key_scale and value_scale must be float8_e8m0fnu");
+    TORCH_CHECK(t->dim() == 3 && t->size(0) == kc.size(0) && t->size(1) == kc.size(1) && t->size(2) == kc.size(2),
+                "key_scale and value_scale must be (Pages, Heads, Page size)");
+    TORCH_CHECK(t->device() == like.device(), "Device mismatch");
+  }
+  return CMPX_E4M3;
+}
+
+// The same for queries over a paged cache: key_cache / value_cache
+// [pages, Hkv, page_size, D] in the query's dtype or float8_e4m3fn with
+// float8_e8m0fnu scales [pages, Hkv, page_size].
+torch::Tensor attention_paged(torch::Tensor query, torch::Tensor key_cache, torch::Tensor value_cache,
+                              torch::Tensor page_table, torch::Tensor seqlens_k,
+                              c10::optional<torch::Tensor> cu_seqlens_q, bool causal, c10::optional<double> scale,
+                              c10::optional<torch::Tensor> key_scale, c10::optional<torch::Tensor> value_scale,
+                              c10::optional<int64_t> max_seqlen_q, c10::optional<torch::Tensor> out_arg) {
+  TORCH_CHECK(query.dim() == 3, "Query must be 3D (Tokens, Heads, Dim)");
+  const int64_t D = query.size(2);
+  const int dt = dtype_code(query.scalar_type());
+  const int kv = check_cache(key_cache, value_cache, key_scale, value_scale, -1, D, query);
+  const int64_t Hkv = key_cache.size(1);
+  TORCH_CHECK(query.size(1) == 0 || (Hkv > 0 && query.size(1) % Hkv == 0),
+              "Query heads must be a multiple of key_cache heads");
+  TORCH_CHECK(dt >= 0, "Unsupported dtype for attention");
+  TORCH_CHECK(kv == CMPX_E4M3 || key_cache.scalar_type() == query.scalar_type(), "Dtype mismatch");
+  TORCH_CHECK(page_table.dim() == 2, "page_table must be 2D (Batch, Pages of a sequence)");
+  TORCH_CHECK(page_table.scalar_type() == at::kInt, "page_table must be int32");
+  TORCH_CHECK(page_table.device() == query.device(), "Device mismatch");
+  const int64_t B = page_table.size(0);
+  torch::Tensor lens = index_arg(seqlens_k, "seqlens_k", B, query);
+  torch::Tensor cu_q;
+  if (cu_seqlens_q.has_value() && cu_seqlens_q->defined())
+    cu_q = index_arg(*cu_seqlens_q, "cu_seqlens_q", B + 1, query);
+  else
+    TORCH_CHECK(B == 0 ? query.size(0) == 0 : query.size(0) % B == 0,
+                "Without cu_seqlens_q, every sequence has the same number of query tokens");
+  TORCH_CHECK(!max_seqlen_q.has_value() || *max_seqlen_q >= 0, "max_seqlen_q must not be negative");
+  TORCH_CHECK(query.is_cuda(), "attention_paged expects CUDA tensors");
+  c10::cuda::CUDAGuard guard(query.device());
+  torch::Tensor out = seq_output(out_arg, query,
+                                 {query, key_cache, value_cache, page_table, seqlens_k, cu_q,
+                                  kv == CMPX_E4M3 ? *key_scale : torch::Tensor(),
+                                  kv == CMPX_E4M3 ? *value_scale : torch::Tensor()});
+  query = rows16(query);
+  lens = lens.contiguous();
+  if (cu_q.defined()) cu_q = cu_q.contiguous();
+  if (page_table.size(1) > 1 && page_table.stride(1) != 1) page_table = page_table.contiguous();
+  cmpx_attention_seq_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.dtype = dt;
+  a.kv_dtype = kv;
+  set_query(a, query, out);
+  a.K = key_cache.data_ptr();
+  a.V = value_cache.data_ptr();
+  a.batch = B;
+  a.heads_kv = Hkv;
+  a.pages = key_cache.size(0);
+  a.page_size = key_cache.size(2);
+  a.k_stride_row = stride_or(key_cache, 2, D);
+  a.k_stride_head = stride_or(key_cache, 1, D * a.page_size);
+  a.k_stride_page = stride_or(key_cache, 0, D * a.page_size * Hkv);
+  a.v_stride_row = stride_or(value_cache, 2, D);
+  a.v_stride_head = stride_or(value_cache, 1, D * a.page_size);
+  a.v_stride_page = stride_or(value_cache, 0, D * a.page_size * Hkv);
+  if (kv == CMPX_E4M3) {
+    a.k_scale = key_scale->data_ptr();
+    a.v_scale = value_scale->data_ptr();
+    a.ks_stride_page = key_scale->stride(0);
+    a.ks_stride_head = key_scale->stride(1);
+    a.ks_stride_row = key_scale->stride(2);
+    a.vs_stride_page = value_scale->stride(0);
+    a.vs_stride_head = value_scale->stride(1);
+    a.vs_stride_row = value_scale->stride(2);
+  }
+  // an empty page table still marks the paged form
+  static const int no_pages = 0;
+  a.page_table = page_table.numel() > 0 ? page_table.data_ptr<int>() : &no_pages;
+  a.page_table_stride = page_table.size(1) > 0 ? stride_or(page_table, 0, page_table.size(1)) : 0;
+  a.max_pages = page_table.size(1);
+  a.seqlens_k = B > 0 ? lens.data_ptr<int>() : &no_pages;
+  a.cu_seqlens_q = cu_q.defined() ? cu_q.data_ptr<int>() : nullptr;
+  a.max_seqlen_q = max_seqlen_q.has_value() ? *max_seqlen_q : 0;
+  a.scale = seq_scale(scale, D);
+  a.causal = causal;
+  a.zero_rest = !(out_arg.has_value() && out_arg->defined());
+  run_seq(a, query, "attention_paged");
+  return out;
+}
+
+void set_cache(cmpx_kv_cache_args& a, const torch::Tensor& kc, const torch::Tensor& vc,
+               const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs) {
+  a.key_cache = kc.data_ptr();
+  a.value_cache = vc.data_ptr();
+  a.pages = kc.size(0);
+  a.heads = kc.size(1);
+  a.page_size = kc.size(2);
+  a.head_dim = kc.size(3);
+  a.kc_stride_page = kc.stride(0);
+  a.kc_stride_head = kc.stride(1);
+  a.kc_stride_row = kc.stride(2);
+  a.vc_stride_page = vc.stride(0);
+  a.vc_stride_head = vc.stride(1);
+  a.vc_stride_row = vc.stride(2);
+  if (a.cache_dtype == CMPX_E4M3) {
+    a.key_scale = ks->data_ptr();
+    a.value_scale = vs->data_ptr();
+    a.ks_stride_page = ks->stride(0);
+    a.ks_stride_head = ks->stride(1);
+    a.ks_stride_row = ks->stride(2);
+    a.vs_stride_page = vs->stride(0);
+    a.vs_stride_head = vs->stride(1);
+    a.vs_stride_row = vs->stride(2);
+  }
+}
+
+void check_slots(const torch::Tensor& slots, const torch::Tensor& like) {
+  TORCH_CHECK(slots.dim() == 1, "slots must be 1D");
+  TORCH_CHECK(slots.scalar_type() == at::kLong, "slots must be int64");
+  TORCH_CHECK(slots.device() == like.device(), "Device mismatch");
+}
+
+// Writes key / value [T, Hkv, D] to slots[t] = page * page_size + offset of
+// the caches, quantised where they are float8_e4m3fn.
+void kv_cache_write(torch::Tensor key, torch::Tensor value, torch::Tensor key_cache, torch::Tensor value_cache,
+                    torch::Tensor slots, c10::optional<torch::Tensor> key_scale,
+                    c10::optional<torch::Tensor> value_scale) {
+  TORCH_CHECK(key.dim() == 3, "Key must be 3D (Tokens, Heads, Dim)");
+  TORCH_CHECK(value.sizes() == key.sizes(), "Value shape mismatch");
+  TORCH_CHECK(key.device() == value.device(), "Device mismatch");
+  TORCH_CHECK(value.scalar_type() == key.scalar_type(), "Dtype mismatch");
+  const int dt = dtype_code(key.scalar_type());
+  TORCH_CHECK(dt >= 0, "Unsupported dtype for kv_cache_write");
+  const int kv = check_cache(key_cache, value_cache, key_scale, value_scale, key.size(1), key.size(2), key);
+  TORCH_CHECK(kv == dt || kv == CMPX_E4M3, "Dtype mismatch");
+  check_slots(slots, key);
+  TORCH_CHECK(slots.size(0) == key.size(0), "slots must have one element for each token");
+  std::vector<std::pair<torch::Tensor, const char*>> written = {{key_cache, "key_cache"}, {value_cache, "value_cache"}};
+  if (kv == CMPX_E4M3) {
+    written.emplace_back(*key_scale, "key_scale");
+    written.emplace_back(*value_scale, "value_scale");
+  }
+  for (size_t i = 0; i < written.size(); ++i) {
+    check_writable(written[i].first, written[i].second, i < 2);
+    for (size_t j = 0; j < i; ++j)
+      TORCH_CHECK(written[i].first.numel() == 0 || written[i].first.data_ptr() != written[j].first.data_ptr(),
+                  written[i].second, " must not be ", written[j].second);
+  }
+  TORCH_CHECK(key.is_cuda(), "kv_cache_write expects CUDA tensors");
+  c10::cuda::CUDAGuard guard(key.device());
+  if (key.numel() > 0 && key.stride(2) != 1) key = key.contiguous();
+  if (value.numel() > 0 && value.stride(2) != 1) value = value.contiguous();
+  slots = slots.contiguous();
+  cmpx_kv_cache_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.dtype = dt;
+  a.cache_dtype = kv;
+  set_cache(a, key_cache, value_cache, key_scale, value_scale);
+  a.key = key.data_ptr();
+  a.value = value.data_ptr();
+  a.tokens = key.size(0);
+  a.slots = slots.data_ptr<int64_t>();
+  a.key_stride_token = key.stride(0);
+  a.key_stride_head = key.stride(1);
+  a.value_stride_token = value.stride(0);
+  a.value_stride_head = value.stride(1);
+  check_status(cmpx_kv_cache_write(&a, current_stream()), "kv_cache_write");
+}
+
+// The tokens at `slots` as (key, value) [T, Hkv, D] in `dtype` (a 16- or
+// 32-bit cache's own dtype; float8_e4m3fn: bfloat16 unless given).
+std::tuple<torch::Tensor, torch::Tensor> kv_cache_read(torch::Tensor key_cache, torch::Tensor value_cache,
+                                                       torch::Tensor slots, c10::optional<torch::Tensor> key_scale,
+                                                       c10::optional<torch::Tensor> value_scale, py::object dtype) {
+  const int kv = check_cache(key_cache, value_cache, key_scale, value_scale, -1, -1, key_cache);
+  TORCH_CHECK(kv >= 0, "Unsupported dtype for kv_cache_read");
+  at::ScalarType want = kv == CMPX_E4M3 ? at::kBFloat16 : key_cache.scalar_type();
+  if (!dtype.is_none()) want = torch::python::detail::py_object_to_dtype(dtype);
+  const int dt = dtype_code(want);
+  TORCH_CHECK(dt >= 0, "Unsupported dtype for kv_cache_read");
+  TORCH_CHECK(kv == dt || kv == CMPX_E4M3, "Dtype mismatch");
+  check_slots(slots, key_cache);
+  TORCH_CHECK(key_cache.is_cuda(), "kv_cache_read expects CUDA tensors");
+  c10::cuda::CUDAGuard guard(key_cache.device());
+  slots = slots.contiguous();
+  torch::Tensor key = torch::empty({slots.size(0), key_cache.size(1), key_cache.size(3)},
+                                   key_cache.options().dtype(want));
+  torch::Tensor value = torch::empty_like(key);
+  cmpx_kv_cache_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.dtype = dt;
+  a.cache_dtype = kv;
+  set_cache(a, key_cache, value_cache, key_scale, value_scale);
+  a.key = key.data_ptr();
+  a.value = value.data_ptr();
+  a.tokens = slots.size(0);
+  a.slots = slots.data_ptr<int64_t>();
+  a.key_stride_token = key.stride(0);
+  a.key_stride_head = key.stride(1);
+  a.value_stride_token = value.stride(0);
+  a.value_stride_head = value.stride(1);
+  check_status(cmpx_kv_cache_read(&a, current_stream()), "kv_cache_read");
+  return {key, value};
+}
+
 torch::Tensor fp16_matmul(torch::Tensor a, torch::Tensor b) { return matmul_2d(a, b, at::kHalf, "fp16_matmul"); }
 torch::Tensor bf16_matmul(torch::Tensor a, torch::Tensor b) { return matmul_2d(a, b, at::kBFloat16, "bf16_matmul"); }
 torch::Tensor fp32_matmul(torch::Tensor a, torch::Tensor b) { return matmul_2d(a, b, at::kFloat, "fp32_matmul"); }
@@ -438,6 +825,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("b"), py::arg("out"), py::arg("peer_out") = std::vector<int64_t>{}, py::arg("mc_out") = 0);
   m.def("attention", &attention, "scaled dot-product attention (cmpext3.attention)", py::arg("query"),
         py::arg("key"), py::arg("value"), py::arg("scale") = py::none());
+  m.def("attention_varlen", &attention_varlen,
+        "attention over sequences packed along the token dimension, grouped heads, causal", py::arg("query"),
+        py::arg("key"), py::arg("value"), py::arg("cu_seqlens_q"), py::arg("cu_seqlens_k") = py::none(),
+        py::arg("causal") = true, py::arg("scale") = py::none(), py::arg("out") = py::none());
+  m.def("attention_paged", &attention_paged, "attention of new tokens over a paged key / value cache",
+        py::arg("query"), py::arg("key_cache"), py::arg("value_cache"), py::arg("page_table"), py::arg("seqlens_k"),
+        py::arg("cu_seqlens_q") = py::none(), py::arg("causal") = true, py::arg("scale") = py::none(),
+        py::arg("key_scale") = py::none(), py::arg("value_scale") = py::none(), py::arg("max_seqlen_q") = py::none(),
+        py::arg("out") = py::none());
+  m.def("kv_cache_write", &kv_cache_write, "new tokens' keys and values into a paged cache (in place)",
+        py::arg("key"), py::arg("value"), py::arg("key_cache"), py::arg("value_cache"), py::arg("slots"),
+        py::arg("key_scale") = py::none(), py::arg("value_scale") = py::none());
+  m.def("kv_cache_read", &kv_cache_read, "(key, value) of the tokens at slots of a paged cache", py::arg("key_cache"),
+        py::arg("value_cache"), py::arg("slots"), py::arg("key_scale") = py::none(),
+        py::arg("value_scale") = py::none(), py::arg("dtype") = py::none());
   m.def("_matmul_gather_ce", &matmul_gather_ce,
         "a @ b into out with the rows copied to peer outputs on copy streams as tile columns finish (internal)",
         py::arg("a"), py::arg("b"), py::arg("out"), py::arg("peer_out"), py::arg("flags"), py::arg("n_groups"),

@@ -61,7 +61,12 @@ typedef enum {
   CMPX_ERR_TOO_LARGE = 7    /* problem exceeds the fixed scratch of cmpx_matmul_skinny_noalloc() */
 } cmpx_status;
 
-typedef enum { CMPX_F16 = 0, CMPX_BF16 = 1, CMPX_F32 = 2 } cmpx_dtype;
+typedef enum {
+  CMPX_F16 = 0,
+  CMPX_BF16 = 1,
+  CMPX_F32 = 2,
+  CMPX_E4M3 = 3 /* 8-bit key / value caches only (kv_dtype) */
+} cmpx_dtype;
 
 typedef enum {
   CMPX_B_KN = 0, /* B is [K, N] row-major (matmul / bmm operand, reference layout) */
@@ -221,6 +226,106 @@ CMPX_API int cmpx_attention(int dtype, const void* Q, const void* K, const void*
 /* Which attention path cmpx_attention would take (cmpx_path value), or -1. */
 CMPX_API int cmpx_attention_select_path(int dtype, const void* Q, const void* K, const void* V, const void* O,
                                         int64_t D, int path);
+
+/* Attention for serving language models: packed sequences of different
+ * lengths, grouped heads, causal masks, keys and values packed like the
+ * queries or in a paged cache.  No counterpart in the reference, whose
+ * attention (above) has one length, no mask and no cache.
+ *
+ * For query token i of a sequence with n new tokens and L keys, query head h
+ * and kv head h / (heads_q / heads_kv):
+ *   O_i = sum_j softmax_j(scale * Q_i . K_j) V_j  over the visible keys j:
+ *   j < L, and with `causal` also j <= L - n + i (the last query sees every
+ *   key).  A row that sees no key (L = 0, or i < n - L) or whose visible
+ *   scores are all -inf gets zeros.  Keys, values and page-table entries that
+ *   no query of a sequence sees never change its rows, NaN and infinities
+ *   among them.
+ *
+ * Softmax statistics and sums are fp32; the output is rounded once.  fp16 /
+ * bf16 with head_dim 64 or 128 run tensor-core kernels (a flash-decoding
+ * kernel for few query rows per kv head, a tcgen05 kernel for more; softmax
+ * weights are rounded to 16 bits once); fp32 and other head_dim up to 512, or
+ * layouts TMA cannot describe, run a CUDA-core kernel.
+ *
+ * All strides are in elements.  The element stride within a head is 1. */
+typedef struct {
+  int dtype;    /* of Q and O: CMPX_F16, CMPX_BF16 or CMPX_F32 */
+  int kv_dtype; /* of K and V: dtype, or CMPX_E4M3 (paged form only) */
+  const void* Q; /* [tokens_q][heads_q][head_dim] */
+  const void* K; /* packed: [tokens_kv][heads_kv][head_dim]; paged: [pages][heads_kv][page_size][head_dim] */
+  const void* V;
+  void* O; /* [tokens_q][heads_q][head_dim]; may not overlap the inputs */
+  int64_t batch, tokens_q, heads_q, heads_kv, head_dim; /* heads_q a multiple of heads_kv */
+  int64_t q_stride_token, q_stride_head, o_stride_token, o_stride_head;
+  int64_t k_stride_row, k_stride_head, v_stride_row, v_stride_head; /* row: token, or slot of a page */
+  const int* cu_seqlens_q; /* device [batch + 1]: first query token of each sequence, ascending; NULL: every sequence
+                              has tokens_q / batch tokens */
+  /* packed form (page_table NULL) */
+  int64_t tokens_kv;
+  const int* cu_seqlens_k; /* device [batch + 1]; NULL: cu_seqlens_q */
+  /* paged form */
+  const int* page_table;   /* device [batch][max_pages]: page of each page_size keys */
+  const int* seqlens_k;    /* device [batch]: keys of each sequence, its new tokens among them */
+  int64_t page_table_stride, max_pages, pages, page_size;
+  int64_t k_stride_page, v_stride_page;
+  const void* k_scale;     /* CMPX_E4M3: e8m0 scales [pages][heads_kv][page_size], one for each key / value vector */
+  const void* v_scale;
+  int64_t ks_stride_page, ks_stride_head, ks_stride_row, vs_stride_page, vs_stride_head, vs_stride_row;
+  float scale;
+  int causal;
+  int zero_rest;        /* 1: rows of O outside every sequence are zeroed; 0: they are left as they were */
+  int64_t max_seqlen_q; /* longest sequence's new tokens if known (picks the kernel, never the result); 0: unknown */
+  int path;             /* CMPX_PATH_AUTO, CMPX_PATH_TC (tcgen05), CMPX_PATH_SKINNY (flash decoding), CMPX_PATH_SIMT */
+  void* workspace;      /* device, 16-byte aligned, cmpx_attention_seq_workspace_size() bytes (NULL if that is 0);
+                           contents need no preparation and do not survive the call */
+  size_t workspace_bytes;
+} cmpx_attention_seq_args;
+
+/* Runs the packed (page_table NULL) or the paged form.  Lengths and page
+ * numbers are read on the device: out-of-range ones are clamped, and a key
+ * whose page number is outside [0, pages) reads as zeros. */
+CMPX_API int cmpx_attention_seq(const cmpx_attention_seq_args* args, cmpx_stream_t stream);
+
+/* Workspace bytes cmpx_attention_seq needs on the current device (partial
+ * results of sequences whose keys are split among thread blocks). */
+CMPX_API size_t cmpx_attention_seq_workspace_size(const cmpx_attention_seq_args* args);
+
+/* Which path cmpx_attention_seq would take (cmpx_path value), or -1. */
+CMPX_API int cmpx_attention_seq_select_path(const cmpx_attention_seq_args* args);
+
+/* New tokens' keys and values written to, or tokens read from, a paged cache.
+ *
+ * slots[t] = page * page_size + offset is token t's place.  A slot outside
+ * the cache (a negative one, say) is skipped by the write and gives zeros in
+ * the read.  Slots of one write must differ: what a slot named twice then
+ * holds is not specified.
+ *
+ * cache_dtype == dtype copies.  cache_dtype CMPX_E4M3 quantises each vector x
+ * of head_dim values: with a = max|x|, e the smallest integer >= -127 with
+ * a <= 448 * 2^e (e = 0 when a = 0), the cache gets e4m3(x * 2^-e), rounded to
+ * nearest even, and the e8m0 scale byte e + 127; a vector that holds a NaN or
+ * an infinity gets the scale byte 255 (NaN) and reads back as NaN.  Scaling by
+ * a power of two is exact, so the only rounding is e4m3's.  The read gives
+ * code * 2^e rounded to dtype, finite values beyond dtype's largest one (e4m3
+ * may round a vector's top up to the next power of two) as that one. */
+typedef struct {
+  int dtype;       /* of key / value: CMPX_F16, CMPX_BF16 or CMPX_F32 */
+  int cache_dtype; /* dtype or CMPX_E4M3 */
+  void* key;       /* [tokens][heads][head_dim]: input of the write, output of the read */
+  void* value;
+  void* key_cache; /* [pages][heads][page_size][head_dim] */
+  void* value_cache;
+  void* key_scale; /* [pages][heads][page_size], CMPX_E4M3 only */
+  void* value_scale;
+  const int64_t* slots; /* device [tokens] */
+  int64_t tokens, heads, head_dim, pages, page_size;
+  int64_t key_stride_token, key_stride_head, value_stride_token, value_stride_head;
+  int64_t kc_stride_page, kc_stride_head, kc_stride_row, vc_stride_page, vc_stride_head, vc_stride_row;
+  int64_t ks_stride_page, ks_stride_head, ks_stride_row, vs_stride_page, vs_stride_head, vs_stride_row;
+} cmpx_kv_cache_args;
+
+CMPX_API int cmpx_kv_cache_write(const cmpx_kv_cache_args* args, cmpx_stream_t stream);
+CMPX_API int cmpx_kv_cache_read(const cmpx_kv_cache_args* args, cmpx_stream_t stream);
 
 /* Reads and clears the device-side error word of the current device
  * (synchronises the device).  *code receives the first error a kernel

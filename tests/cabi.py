@@ -13,7 +13,7 @@ REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(REPO, "cmp_ext_b200", "libcmpx.so")
 HEADER = os.path.join(REPO, "include", "cmpx.h")
 
-F16, BF16, F32 = 0, 1, 2
+F16, BF16, F32, E4M3 = 0, 1, 2, 3
 B_KN, B_NK = 0, 1
 PATH_AUTO, PATH_TC, PATH_SKINNY, PATH_SIMT, PATH_BF16X3 = 0, 1, 2, 3, 4
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_NO_MEMORY, ERR_DEVICE, ERR_WORKSPACE, ERR_TOO_LARGE = range(8)
@@ -47,6 +47,31 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+def _struct(name, text):
+    """A ctypes structure from "type: field, field; ..." (i int, l int64, p pointer, f float, z size_t)."""
+    kinds = {"i": ctypes.c_int, "l": ctypes.c_int64, "p": ctypes.c_void_p, "f": ctypes.c_float, "z": ctypes.c_size_t}
+    fields = []
+    for part in text.split(";"):
+        kind, names = part.split(":")
+        fields += [(n.strip(), kinds[kind.strip()]) for n in names.split(",")]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+AttentionSeqArgs = _struct("AttentionSeqArgs", """
+    i: dtype, kv_dtype; p: Q, K, V, O; l: batch, tokens_q, heads_q, heads_kv, head_dim,
+    q_stride_token, q_stride_head, o_stride_token, o_stride_head,
+    k_stride_row, k_stride_head, v_stride_row, v_stride_head; p: cu_seqlens_q; l: tokens_kv;
+    p: cu_seqlens_k, page_table, seqlens_k; l: page_table_stride, max_pages, pages, page_size,
+    k_stride_page, v_stride_page; p: k_scale, v_scale; l: ks_stride_page, ks_stride_head, ks_stride_row,
+    vs_stride_page, vs_stride_head, vs_stride_row; f: scale; i: causal, zero_rest; l: max_seqlen_q; i: path;
+    p: workspace; z: workspace_bytes""")
+
+KVCacheArgs = _struct("KVCacheArgs", """
+    i: dtype, cache_dtype; p: key, value, key_cache, value_cache, key_scale, value_scale, slots;
+    l: tokens, heads, head_dim, pages, page_size, key_stride_token, key_stride_head, value_stride_token,
+    value_stride_head, kc_stride_page, kc_stride_head, kc_stride_row, vc_stride_page, vc_stride_head, vc_stride_row,
+    ks_stride_page, ks_stride_head, ks_stride_row, vs_stride_page, vs_stride_head, vs_stride_row""")
+
 _lib = None
 
 
@@ -77,6 +102,14 @@ def lib():
         L.cmpx_gemm_gather_ce.argtypes = [ctypes.POINTER(GemmArgs), ctypes.POINTER(ctypes.c_void_p), ctypes.c_int,
                                           ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_uint, ctypes.c_void_p,
                                           ctypes.POINTER(ctypes.c_void_p), ctypes.c_int]
+        for name in ("cmpx_attention_seq", "cmpx_kv_cache_write", "cmpx_kv_cache_read"):
+            f = getattr(L, name)
+            f.restype = ctypes.c_int
+            f.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        L.cmpx_attention_seq_workspace_size.restype = ctypes.c_size_t
+        L.cmpx_attention_seq_workspace_size.argtypes = [ctypes.c_void_p]
+        L.cmpx_attention_seq_select_path.restype = ctypes.c_int
+        L.cmpx_attention_seq_select_path.argtypes = [ctypes.c_void_p]
         _lib = L
     return _lib
 
