@@ -173,13 +173,6 @@ int validate_seq(const cmpx_attention_seq_args* a, bool* empty) {
   return CMPX_OK;
 }
 
-// The kernel that runs a checked, non-empty problem, or -1.
-int seq_path(const cmpx_attention_seq_args* a) {
-  const bool simt_ok = a->head_dim <= kSimtMaxD && (a->tokens_q * a->heads_q + 3) / 4 <= INT_MAX;
-  if (a->path == CMPX_PATH_AUTO || a->path == CMPX_PATH_SIMT) return simt_ok ? CMPX_PATH_SIMT : -1;
-  return -1;
-}
-
 SeqProblem resolve_seq(const cmpx_attention_seq_args* a) {
   SeqProblem p = {};
   p.Q = a->Q;
@@ -216,6 +209,20 @@ SeqProblem resolve_seq(const cmpx_attention_seq_args* a) {
   return p;
 }
 
+// The kernel that runs a checked, non-empty problem, or -1.
+int seq_path(const cmpx_attention_seq_args* a, const SeqProblem& p) {
+  const bool simt_ok = a->head_dim <= kSimtMaxD && (a->tokens_q * a->heads_q + 3) / 4 <= INT_MAX;
+  const bool tile_ok = seq_tile_ok(p, a->dtype, a->kv_dtype);
+  if (a->path == CMPX_PATH_SIMT) return simt_ok ? CMPX_PATH_SIMT : -1;
+  if (a->path == CMPX_PATH_TC) return tile_ok ? CMPX_PATH_TC : -1;
+  if (a->path == CMPX_PATH_SKINNY) return -1;
+  return tile_ok ? CMPX_PATH_TC : simt_ok ? CMPX_PATH_SIMT : -1;
+}
+
+size_t seq_workspace(const SeqProblem& p, int path, const DeviceInfo& dev) {
+  return path == CMPX_PATH_TC ? seq_tile_workspace(p, dev) : 0;
+}
+
 }  // namespace
 
 cudaError_t launch_seq_simt(const SeqProblem& p, int dtype, int kv_dtype, cudaStream_t s) {
@@ -236,25 +243,35 @@ extern "C" int cmpx_attention_seq(const cmpx_attention_seq_args* args, cmpx_stre
   bool empty = false;
   int st = validate_seq(args, &empty);
   if (st != CMPX_OK || empty) return st;
-  const int path = seq_path(args);
+  const SeqProblem p = resolve_seq(args);
+  const int path = seq_path(args, p);
   if (path < 0) return CMPX_ERR_UNSUPPORTED;
   DeviceInfo dev;
   int* err = nullptr;
   st = device_facts(&dev, &err);
   if (st != CMPX_OK) return st;
-  const SeqProblem p = resolve_seq(args);
-  const cudaError_t e = launch_seq_simt(p, args->dtype, args->kv_dtype, stream);
+  const size_t need = seq_workspace(p, path, dev);
+  if (need > 0 && (args->workspace == nullptr || reinterpret_cast<uintptr_t>(args->workspace) % 16 != 0))
+    return CMPX_ERR_INVALID_ARG;
+  if (args->workspace_bytes < need) return CMPX_ERR_WORKSPACE;
+  const cudaError_t e =
+      path == CMPX_PATH_TC ? launch_seq_tile(p, args->dtype, args->kv_dtype, args->workspace, dev, err, stream)
+                           : launch_seq_simt(p, args->dtype, args->kv_dtype, stream);
   return e == cudaSuccess ? CMPX_OK : CMPX_ERR_CUDA;
 }
 
 extern "C" size_t cmpx_attention_seq_workspace_size(const cmpx_attention_seq_args* args) {
   bool empty = false;
   if (validate_seq(args, &empty) != CMPX_OK || empty) return 0;
-  return 0;
+  const SeqProblem p = resolve_seq(args);
+  DeviceInfo dev;
+  int* err = nullptr;
+  if (device_facts(&dev, &err) != CMPX_OK) return 0;
+  return seq_workspace(p, seq_path(args, p), dev);
 }
 
 extern "C" int cmpx_attention_seq_select_path(const cmpx_attention_seq_args* args) {
   bool empty = false;
   if (validate_seq(args, &empty) != CMPX_OK) return -1;
-  return empty ? CMPX_PATH_SIMT : seq_path(args);
+  return empty ? CMPX_PATH_SIMT : seq_path(args, resolve_seq(args));
 }

@@ -77,4 +77,10 @@ __device__ __forceinline__ int2 seq_rest(const SeqProblem& p) {
 // Host side of the kernels.  Each returns a cudaError_t of its launches.
 cudaError_t launch_seq_simt(const SeqProblem& p, int dtype, int kv_dtype, cudaStream_t s);
 
+// tcgen05 kernel (attention_tile.cu)
+bool seq_tile_ok(const SeqProblem& p, int dtype, int kv_dtype);
+size_t seq_tile_workspace(const SeqProblem& p, const DeviceInfo& dev);
+cudaError_t launch_seq_tile(const SeqProblem& p, int dtype, int kv_dtype, void* ws, const DeviceInfo& dev, int* err,
+                            cudaStream_t s);
+
 }  // namespace cmpx
