@@ -28,7 +28,8 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["cmpx_api.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_skinny.cu", "gemm_simt.cu", "cmpx_selftest.cu", "gather_ce.cu",
-              "attention.cu", "attention_seq.cu", "attention_tile.cu", "kv_cache.cu"]
+              "attention.cu", "attention_seq.cu", "attention_tile.cu",
+              "attention_decode.cu", "kv_cache.cu"]
 HEADERS = ["ptx.cuh", "internal.h", "attention_math.cuh", "attention_seq.h"]
 LIB = os.path.join(HERE, "libcmpx.so")
 SHIM_SRC = os.path.join(CSRC, "torch_shim.cpp")

@@ -209,21 +209,66 @@ SeqProblem resolve_seq(const cmpx_attention_seq_args* a) {
   return p;
 }
 
-// The kernel that runs a checked, non-empty problem, or -1.
+// The kernel that runs a checked, non-empty problem, or -1.  Few query rows a
+// kv head run the flash-decoding kernel, whose blocks take 16 of them; more
+// the tcgen05 kernel.  Without a hint the mean length decides.
 int seq_path(const cmpx_attention_seq_args* a, const SeqProblem& p) {
   const bool simt_ok = a->head_dim <= kSimtMaxD && (a->tokens_q * a->heads_q + 3) / 4 <= INT_MAX;
   const bool tile_ok = seq_tile_ok(p, a->dtype, a->kv_dtype);
+  const bool decode_ok = seq_decode_ok(p, a->dtype, a->kv_dtype);
   if (a->path == CMPX_PATH_SIMT) return simt_ok ? CMPX_PATH_SIMT : -1;
   if (a->path == CMPX_PATH_TC) return tile_ok ? CMPX_PATH_TC : -1;
-  if (a->path == CMPX_PATH_SKINNY) return -1;
+  if (a->path == CMPX_PATH_SKINNY) return decode_ok ? CMPX_PATH_SKINNY : -1;
+  const int64_t longest = a->cu_seqlens_q == nullptr ? p.uniform_n
+                          : a->max_seqlen_q > 0      ? a->max_seqlen_q
+                          : a->batch > 0             ? (a->tokens_q + a->batch - 1) / a->batch
+                                                     : 0;
+  if (decode_ok && (longest * p.group <= 16 || !tile_ok)) return CMPX_PATH_SKINNY;
   return tile_ok ? CMPX_PATH_TC : simt_ok ? CMPX_PATH_SIMT : -1;
 }
 
 size_t seq_workspace(const SeqProblem& p, int path, const DeviceInfo& dev) {
-  return path == CMPX_PATH_TC ? seq_tile_workspace(p, dev) : 0;
+  return path == CMPX_PATH_TC ? seq_tile_workspace(p, dev) : path == CMPX_PATH_SKINNY ? seq_decode_workspace(p, dev) : 0;
 }
 
 }  // namespace
+
+bool seq_rows_ok(const void* base, int64_t stride, int64_t count, int64_t unit) {
+  return reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
+         (count <= 1 || (stride > 0 && stride % unit == 0 && stride < (int64_t(1) << 38)));
+}
+
+bool seq_tma_ok(const SeqProblem& p, int kv_dtype) {
+  const bool paged = p.table != nullptr;
+  if (paged && (p.page_size < 8 || (p.page_size & (p.page_size - 1)) != 0)) return false;
+  if (paged ? (p.pages == 0 || p.max_keys == 0) : p.tokens_kv == 0) return false;  // no key at all
+  const int64_t unit = kv_dtype == CMPX_E4M3 ? 16 : 8;
+  for (const SeqKV* x : {&p.k, &p.v}) {
+    if (!seq_rows_ok(x->base, x->row, paged ? p.page_size : p.tokens_kv, unit) ||
+        !seq_rows_ok(x->base, x->head, p.heads_kv, unit) || (paged && !seq_rows_ok(x->base, x->page, p.pages, unit)))
+      return false;
+  }
+  return true;
+}
+
+bool seq_rows_map(CUtensorMap* m, int dtype, const void* base, const uint64_t (&dims)[4], const int64_t (&strides)[3],
+                  uint32_t box0, uint32_t box1, uint32_t box3, uint32_t swizzle_bytes) {
+  const uint64_t es = dtype == CMPX_E4M3 ? 1 : 2;
+  uint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) bytes[i] = dims[i + 1] > 1 ? uint64_t(strides[i]) * es : dims[0] * es;
+  return encode_tmap_4d(m, dtype, base, dims, bytes, box0, box1, box3, swizzle_bytes) == CMPX_OK;
+}
+
+bool seq_kv_maps(const SeqProblem& p, int kv_dtype, int box_rows, bool swizzled, CUtensorMap* tk, CUtensorMap* tv) {
+  const bool paged = p.table != nullptr, q8 = kv_dtype == CMPX_E4M3;
+  const uint64_t dims[4] = {uint64_t(p.d), uint64_t(paged ? p.page_size : p.tokens_kv), uint64_t(p.heads_kv),
+                            uint64_t(paged ? p.pages : 1)};
+  const uint32_t inner = q8 ? uint32_t(p.d) : 64u;
+  const uint32_t swizzle = !swizzled ? 0u : q8 ? uint32_t(p.d) : 128u;
+  const int64_t ks[3] = {p.k.row, p.k.head, p.k.page}, vs[3] = {p.v.row, p.v.head, p.v.page};
+  return seq_rows_map(tk, kv_dtype, p.k.base, dims, ks, inner, uint32_t(box_rows), 1, swizzle) &&
+         seq_rows_map(tv, kv_dtype, p.v.base, dims, vs, inner, uint32_t(box_rows), 1, swizzle);
+}
 
 cudaError_t launch_seq_simt(const SeqProblem& p, int dtype, int kv_dtype, cudaStream_t s) {
   if (kv_dtype == CMPX_E4M3)
@@ -255,7 +300,9 @@ extern "C" int cmpx_attention_seq(const cmpx_attention_seq_args* args, cmpx_stre
     return CMPX_ERR_INVALID_ARG;
   if (args->workspace_bytes < need) return CMPX_ERR_WORKSPACE;
   const cudaError_t e =
-      path == CMPX_PATH_TC ? launch_seq_tile(p, args->dtype, args->kv_dtype, args->workspace, dev, err, stream)
+      path == CMPX_PATH_SKINNY
+          ? launch_seq_decode(p, args->dtype, args->kv_dtype, args->workspace, dev, err, stream)
+      : path == CMPX_PATH_TC ? launch_seq_tile(p, args->dtype, args->kv_dtype, args->workspace, dev, err, stream)
                            : launch_seq_simt(p, args->dtype, args->kv_dtype, stream);
   return e == cudaSuccess ? CMPX_OK : CMPX_ERR_CUDA;
 }

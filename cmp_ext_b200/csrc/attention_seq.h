@@ -66,6 +66,11 @@ __device__ __forceinline__ Seq seq_of(const SeqProblem& p, int b) {
 __device__ __forceinline__ int seq_limit(const SeqProblem& p, const Seq& s, int i) {
   return p.causal ? min(max(s.len - s.n + i + 1, 0), s.len) : s.len;
 }
+// Records a bounded wait that ran out and ends the block's other waits.
+__device__ __forceinline__ void rec_err(int* err, volatile int* abort, int code) {
+  *abort = 1;
+  atomicCAS(err, 0, code);
+}
 // First token that no sequence holds any more (cu_seqlens_q[batch], clamped),
 // and the number of tokens before the first sequence.
 __device__ __forceinline__ int2 seq_rest(const SeqProblem& p) {
@@ -76,6 +81,24 @@ __device__ __forceinline__ int2 seq_rest(const SeqProblem& p) {
 
 // Host side of the kernels.  Each returns a cudaError_t of its launches.
 cudaError_t launch_seq_simt(const SeqProblem& p, int dtype, int kv_dtype, cudaStream_t s);
+
+// Whether TMA can describe a stride of `count` rows (in units that make 16
+// bytes), and the keys and values of a problem.
+bool seq_rows_ok(const void* base, int64_t stride, int64_t count, int64_t unit);
+bool seq_tma_ok(const SeqProblem& p, int kv_dtype);
+// 4-D map of rows, innermost dimension first, boxes {box0, box1, 1, box3};
+// a dimension of one element takes any stride.
+bool seq_rows_map(CUtensorMap* m, int dtype, const void* base, const uint64_t (&dims)[4], const int64_t (&strides)[3],
+                  uint32_t box0, uint32_t box1, uint32_t box3, uint32_t swizzle_bytes);
+// Maps of keys and values, boxes of box_rows keys of a head: 16-bit rows in
+// 128-byte columns; 8-bit rows whole, swizzled by their own length or not.
+bool seq_kv_maps(const SeqProblem& p, int kv_dtype, int box_rows, bool swizzled, CUtensorMap* tk, CUtensorMap* tv);
+
+// flash-decoding kernel (attention_decode.cu)
+bool seq_decode_ok(const SeqProblem& p, int dtype, int kv_dtype);
+size_t seq_decode_workspace(const SeqProblem& p, const DeviceInfo& dev);
+cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, void* ws, const DeviceInfo& dev, int* err,
+                              cudaStream_t s);
 
 // tcgen05 kernel (attention_tile.cu)
 bool seq_tile_ok(const SeqProblem& p, int dtype, int kv_dtype);

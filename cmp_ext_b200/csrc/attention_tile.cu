@@ -83,11 +83,6 @@ struct TileParams {
   int* err;
 };
 
-__device__ __forceinline__ void rec_err(int* err, volatile int* abort, int code) {
-  *abort = 1;
-  atomicCAS(err, 0, code);
-}
-
 // A warpgroup's registers a thread, given up to or taken from the block's own.
 template <int N>
 __device__ __forceinline__ void regs_dec() {
@@ -96,38 +91,6 @@ __device__ __forceinline__ void regs_dec() {
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// D[tmem] (+)= A[tmem] * B[smem desc]: A is 128 lanes of packed 16-bit pairs.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Whether the phase is over, without the suspension of try_wait: a thread
-// that polls several barriers must not sleep on one of them.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z,
-                                            int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
 }
 
 // Two e4m3 codes times a scale, in T, saturating.
@@ -455,8 +418,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
             // S of block j: the last product of this tile must be done with
             // P, which lies where S goes
             const int j = qk[t];
-            if (j < n[t] && mbar_test(&k_full[j % KS], (j / KS) & 1) &&
-                (j == 0 || mbar_test(&o_done[t], (j - 1) & 1))) {
+            if (j < n[t] && mbar_test_wait(&k_full[j % KS], (j / KS) & 1) &&
+                (j == 0 || mbar_test_wait(&o_done[t], (j - 1) & 1))) {
               tc_fence_after();
               const uint32_t q_addr = smem_u32(sQ + t * Cfg::TILE);
               const uint32_t k_addr = smem_u32(sK + (j % KS) * Cfg::TILE);
@@ -476,8 +439,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
             }
           } else {
             const int j = pv[t];
-            const bool cleared = Q8 || j + 1 < nkv || last_keys == 128 || mbar_test(tail, 0);
-            if (cleared && mbar_test(&v_full[j % VS], (j / VS) & 1) && mbar_test(&p_full[t], j & 1)) {
+            const bool cleared = Q8 || j + 1 < nkv || last_keys == 128 || mbar_test_wait(tail, 0);
+            if (cleared && mbar_test_wait(&v_full[j % VS], (j / VS) & 1) && mbar_test_wait(&p_full[t], j & 1)) {
               tc_fence_after();
               const uint32_t v_addr = smem_u32(sV + (j % VS) * Cfg::TILE);
               const int steps = j + 1 < nkv ? 8 : (last_keys + 15) >> 4;
@@ -811,16 +774,6 @@ __global__ void __launch_bounds__(128) attention_seq_combine(const SeqProblem p,
 }
 
 // ------------------------------------------------------------------ host
-// 4-D map of 16-bit rows in 128-byte-swizzled boxes, or of 8-bit rows as they
-// are.  A dimension of one element takes any legal stride.
-bool encode_rows(CUtensorMap* m, int dtype, const void* base, const uint64_t (&dims)[4], const int64_t (&strides)[3],
-                 uint32_t box1, uint32_t box3, uint32_t inner) {
-  const uint64_t es = dtype == CMPX_E4M3 ? 1 : 2;
-  uint64_t bytes[3];
-  for (int i = 0; i < 3; ++i) bytes[i] = dims[i + 1] > 1 ? uint64_t(strides[i]) * es : dims[0] * es;
-  return encode_tmap_4d(m, dtype, base, dims, bytes, inner, box1, box3) == CMPX_OK;
-}
-
 template <int FMT, int D, bool Q8>
 cudaError_t launch_tile_typed(const TileParams& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                               int64_t tiles, cudaStream_t s) {
@@ -878,22 +831,9 @@ bool seq_tile_ok(const SeqProblem& p, int dtype, int kv_dtype) {
   if ((dtype != CMPX_F16 && dtype != CMPX_BF16) || (p.d != 64 && p.d != 128) || p.group > 128) return false;
   // masked scores are -inf, which a scale of 0 would turn into NaN
   if (!(p.scale_log2 < 0.0f || p.scale_log2 > 0.0f) || p.scale_log2 - p.scale_log2 != 0.0f) return false;
-  const bool paged = p.table != nullptr;
-  if (paged && (p.page_size < 8 || (p.page_size & (p.page_size - 1)) != 0)) return false;
-  if (paged ? (p.pages == 0 || p.max_keys == 0) : p.tokens_kv == 0) return false;  // no key at all
-  const auto fits = [](const void* base, int64_t stride, int64_t count, int64_t unit) {
-    return reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
-           (count <= 1 || (stride > 0 && stride % unit == 0 && stride < (int64_t(1) << 38)));
-  };
-  const int64_t unit = kv_dtype == CMPX_E4M3 ? 16 : 8;
-  if (!fits(p.Q, p.q_token, p.tokens_q, 8) || !fits(p.Q, p.q_head, p.heads_q, 8)) return false;
-  if (p.q_head * p.group >= (int64_t(1) << 38)) return false;
-  for (const SeqKV* x : {&p.k, &p.v}) {
-    if (!fits(x->base, x->row, paged ? p.page_size : p.tokens_kv, unit) || !fits(x->base, x->head, p.heads_kv, unit) ||
-        (paged && !fits(x->base, x->page, p.pages, unit)))
-      return false;
-  }
-  return tile_count(p) <= 0x7fffffffLL && (int64_t(p.tokens_q) * p.heads_q + 3) / 4 <= 0x7fffffffLL;
+  return seq_tma_ok(p, kv_dtype) && seq_rows_ok(p.Q, p.q_token, p.tokens_q, 8) &&
+         seq_rows_ok(p.Q, p.q_head, p.heads_q, 8) && p.q_head * p.group < (int64_t(1) << 38) &&
+         tile_count(p) <= 0x7fffffffLL && (int64_t(p.tokens_q) * p.heads_q + 3) / 4 <= 0x7fffffffLL;
 }
 
 size_t seq_tile_workspace(const SeqProblem& p, const DeviceInfo& dev) {
@@ -913,15 +853,10 @@ cudaError_t launch_seq_tile(const SeqProblem& p, int dtype, int kv_dtype, void* 
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (a.splits == 1 ? 0 : int64_t(a.splits) * p.tokens_q * p.heads_q * p.d));
   a.err = err;
   CUtensorMap tq, tk, tv;
-  const uint64_t d = uint64_t(p.d), hkv = uint64_t(p.heads_kv);
-  const uint64_t qd[4] = {d, uint64_t(p.group), hkv, uint64_t(p.tokens_q)};
+  const uint64_t qd[4] = {uint64_t(p.d), uint64_t(p.group), uint64_t(p.heads_kv), uint64_t(p.tokens_q)};
   const int64_t qs[3] = {p.q_head, p.q_head * p.group, p.q_token};
-  bool ok = encode_rows(&tq, dtype, p.Q, qd, qs, uint32_t(p.group), uint32_t(a.tokens), 64);
-  const uint64_t kd[4] = {d, uint64_t(paged ? p.page_size : p.tokens_kv), hkv, uint64_t(paged ? p.pages : 1)};
-  const int64_t ks[3] = {p.k.row, p.k.head, p.k.page}, vs[3] = {p.v.row, p.v.head, p.v.page};
-  const uint32_t inner = q8 ? uint32_t(p.d) : 64u;
-  ok = ok && encode_rows(&tk, kv_dtype, p.k.base, kd, ks, uint32_t(a.box_rows), 1, inner);
-  ok = ok && encode_rows(&tv, kv_dtype, p.v.base, kd, vs, uint32_t(a.box_rows), 1, inner);
+  const bool ok = seq_rows_map(&tq, dtype, p.Q, qd, qs, 64, uint32_t(p.group), uint32_t(a.tokens), 128) &&
+                  seq_kv_maps(p, kv_dtype, a.box_rows, !q8, &tk, &tv);
   if (!ok) return cudaErrorInvalidValue;
   const int64_t tiles = tile_count(p);
   if (dtype == CMPX_F16) {

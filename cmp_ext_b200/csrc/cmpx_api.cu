@@ -574,7 +574,8 @@ int encode_tmap_3d(CUtensorMap* m, int dtype, const void* base, uint64_t inner, 
 }
 
 int encode_tmap_4d(CUtensorMap* m, int dtype, const void* base, const uint64_t (&dims)[4],
-                   const uint64_t (&stride_bytes)[3], uint32_t box0, uint32_t box1, uint32_t box3) {
+                   const uint64_t (&stride_bytes)[3], uint32_t box0, uint32_t box1, uint32_t box3,
+                   uint32_t swizzle_bytes) {
   const CUtensorMapDataType dt = dtype == CMPX_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                  : dtype == CMPX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -583,7 +584,9 @@ int encode_tmap_4d(CUtensorMap* m, int dtype, const void* base, const uint64_t (
   cuuint32_t box[4] = {box0, box1, 1, box3};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = g_encode(m, dt, 4, const_cast<void*>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        dtype == CMPX_E4M3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                        swizzle_bytes == 0    ? CU_TENSOR_MAP_SWIZZLE_NONE
+                        : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                              : CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? CMPX_OK : CMPX_ERR_CUDA;
 }

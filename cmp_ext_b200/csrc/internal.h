@@ -142,10 +142,11 @@ int device_facts(DeviceInfo* info, int** err_word);
 int encode_tmap_3d(CUtensorMap* m, int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
                    uint64_t ld, uint64_t bstride, uint32_t box_inner, uint32_t box_rows);
 // 4-D map over dims (innermost first; stride_bytes of the outer three) with
-// boxes {box0, box1, 1, box3}: 128-byte swizzle for 16-bit types, none for
-// CMPX_E4M3.
+// boxes {box0, box1, 1, box3}; dtype a 16-bit type or CMPX_E4M3, swizzle_bytes
+// 0, 64 or 128.
 int encode_tmap_4d(CUtensorMap* m, int dtype, const void* base, const uint64_t (&dims)[4],
-                   const uint64_t (&stride_bytes)[3], uint32_t box0, uint32_t box1, uint32_t box3);
+                   const uint64_t (&stride_bytes)[3], uint32_t box0, uint32_t box1, uint32_t box3,
+                   uint32_t swizzle_bytes);
 
 // Programmatic dependent launch for the GEMM kernels (on unless CMPX_PDL=0).
 bool pdl_enabled();

@@ -19,6 +19,14 @@ F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
+PATHS = ["auto", "simt", "tc", "skinny"]
+
+
+def takes(path, dtype, d, page=8):
+    """Whether a forced kernel takes the case (the tensor-core ones: 16-bit, D 64 or 128, pages of 8, 16, 32, ... keys)."""
+    return path in ("auto", "simt") or (dtype != F32 and d in (64, 128) and page >= 8 and page & (page - 1) == 0)
+
+
 @contextlib.contextmanager
 def forced(path):
     cx._set_path(path)
@@ -67,13 +75,15 @@ LENS = {
 }
 
 
-@pytest.mark.parametrize("path", ["auto", "simt"])
+@pytest.mark.parametrize("path", PATHS)
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype,d,hq,hkv", [(F16, 64, 4, 4), (BF16, 128, 8, 2), (BF16, 64, 7, 1), (F16, 128, 6, 2),
                                             (F32, 64, 2, 1), (BF16, 80, 4, 2), (F16, 128, 5, 1)])
 @pytest.mark.parametrize("lens", list(LENS))
 def test_varlen(cuda, lens, dtype, d, hq, hkv, causal, path):
     lens = LENS[lens]
+    if not takes(path, dtype, d):
+        pytest.skip("not this kernel's")
     q, k, v = qkv(sum(lens), hq, hkv, d, dtype, seed=sum(lens) + d)
     cu = cu_of(lens)
     with forced(path):
@@ -82,15 +92,19 @@ def test_varlen(cuda, lens, dtype, d, hq, hkv, causal, path):
     check_varlen(out, q, k, v, cu, cu, causal, 1 / math.sqrt(d), "varlen")
 
 
+@pytest.mark.parametrize("path", PATHS)
 @pytest.mark.parametrize("dtype,d", [(F16, 64), (BF16, 128), (F32, 40)])
 @pytest.mark.parametrize("causal", [True, False])
-def test_varlen_other_key_lengths(cuda, dtype, d, causal):
+def test_varlen_other_key_lengths(cuda, dtype, d, causal, path):
     """More keys than queries, fewer (rows that see nothing), none."""
+    if not takes(path, dtype, d):
+        pytest.skip("not this kernel's")
     n, length = [5, 130, 40, 3, 200, 1], [300, 7, 0, 3, 129, 1000]
     q, _, _ = qkv(sum(n), 4, 2, d, dtype, 1)
     _, k, v = qkv(sum(length), 4, 2, d, dtype, 2)
     cu_q, cu_k = cu_of(n), cu_of(length)
-    out = cx.attention_varlen(q, k, v, cu_q, cu_k, causal=causal, scale=-0.2)
+    with forced(path):
+        out = cx.attention_varlen(q, k, v, cu_q, cu_k, causal=causal, scale=-0.2)
     finish()
     check_varlen(out, q, k, v, cu_q, cu_k, causal, -0.2, "varlen")
     assert not out[cu_q[2] : cu_q[3]].any()  # no keys: zeros
@@ -121,22 +135,30 @@ def test_varlen_rest_and_garbage_between(cuda, dtype, d):
 
 @pytest.mark.parametrize("dtype,d,hq,hkv", [(F16, 64, 4, 4), (BF16, 128, 8, 1), (F32, 64, 2, 2)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_varlen_bad_values_stay_with_their_keys(cuda, dtype, d, hq, hkv, bad):
+@pytest.mark.parametrize("path", PATHS)
+def test_varlen_bad_values_stay_with_their_keys(cuda, dtype, d, hq, hkv, bad, path):
     """A key or value that is not finite reaches the rows that see it and no
     other.  Other sequences, and every row a bad key is hidden from, keep their
     bits; rows a bad value is hidden from may be summed in another order (the
     bound holds for them)."""
     lens, at = [150, 60], 97
+    if not takes(path, dtype, d):
+        pytest.skip("not this kernel's")
+
+    def run():
+        with forced(path):
+            return cx.attention_varlen(q, k, v, cu_of(lens))
+
     q, k, v = (x.clone() for x in qkv(210, hq, hkv, d, dtype, 4))
-    clean = cx.attention_varlen(q, k, v, cu_of(lens))
+    clean = run()
     v[at, 0, 5] = bad
-    out = cx.attention_varlen(q, k, v, cu_of(lens))
+    out = run()
     finish()
     check_varlen(out, q, k, v, cu_of(lens), cu_of(lens), True, 1 / math.sqrt(d), "value")
     assert out[:at].isfinite().all() and torch.equal(out[150:], clean[150:])
     v[at, 0, 5] = 0
     k[at] = bad
-    out = cx.attention_varlen(q, k, v, cu_of(lens))
+    out = run()
     finish()
     assert torch.equal(out[:at], clean[:at]) and torch.equal(out[150:], clean[150:])
 
@@ -270,7 +292,7 @@ def test_paged_single_tokens(cuda, dtype, d, hq, hkv, page, kv):
     assert torch.equal(c.run(q, cu_seqlens_q=cu_of([1] * len(lens)), max_seqlen_q=1), out)
 
 
-@pytest.mark.parametrize("path", ["auto", "simt"])
+@pytest.mark.parametrize("path", PATHS)
 @pytest.mark.parametrize("kv", ["same", "e4m3"])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype,d,hq,hkv,page", [(F16, 64, 4, 4, 16), (BF16, 128, 8, 2, 32), (F16, 128, 7, 1, 64),
@@ -278,6 +300,8 @@ def test_paged_single_tokens(cuda, dtype, d, hq, hkv, page, kv):
 def test_paged_chunks(cuda, dtype, d, hq, hkv, page, causal, kv, path):
     """Chunks of several lengths in one call: a first chunk (all keys new),
     later ones, single tokens, none, more queries than keys."""
+    if not takes(path, dtype, d, page):
+        pytest.skip("not this kernel's")
     n = [40, 1, 130, 0, 3, 70, 20, 1]
     lens = [40, 500, 333, 64, 1030, 71, 5, 1]
     c = Paged(lens, page, hkv, d, dtype, kv, seed=d + hq)
