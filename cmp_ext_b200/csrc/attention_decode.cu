@@ -3,36 +3,44 @@
 // fp16 / bf16, head_dim 64 or 128, 16-bit or e4m3 keys and values.  No
 // counterpart in the reference.
 //
-// Every key and value is read once for 16 rows, so memory is the bound: at
-// 44 bytes a nanosecond and SM, 128 keys of an e4m3 cache (D = 128) may take
-// 0.75 us, of a 16-bit one 1.5 us.  The products (m16n8k16, rows = token x
-// head of the group, padded to 16) need a fraction of that, so warp-level
-// matrix instructions on registers serve: no tensor-memory round trips in the
-// chain, and 8-bit codes are converted in registers between the load and the
-// product, where the tcgen05 kernel has to write them back to shared memory.
+// Every key and value is read once for the rows of a unit, so memory is the
+// bound: at 44 bytes a nanosecond and SM, 128 keys of an e4m3 cache (D = 128)
+// may take 0.75 us, of a 16-bit one 1.5 us.  The products need a fraction of
+// that, so warp-level matrix instructions on registers serve: no
+// tensor-memory round trips in the chain, and 8-bit codes are converted in
+// registers between the load and the product, where the tcgen05 kernel has to
+// write them back to shared memory.
 //
-// Work: units (sequence, kv head, 16 rows) of ceil(keys / 128) tiles in one
+// The products are turned around: S^T = K Q^T and O^T = V^T P^T, with keys (or
+// output columns) along the 16-wide side of m16n8k16 and query rows (token x
+// head of the group) along the 8-wide one.  Eight rows waste half of what
+// sixteen would, and a warp's state (D x 8 sums) leaves registers for sixteen
+// warps an SM, which is what hides the latency of the strip's chain of
+// dependent steps (with rows along the 16-wide side, twice the products and
+// eight warps, an e4m3 tile took 5200 cycles, now NNNN).
+//
+// Work: units (sequence, kv head, ROWS rows) of ceil(keys / 64) tiles in one
 // list of W tiles; block c of P takes tiles [c W / P, (c + 1) W / P), so
 // ragged lengths and few sequences load every SM alike, and its loads run
 // ahead across unit borders.  A unit that lies in one block is finished
 // there; the pieces of the others (at most two a block) go to the workspace
 // and attention_decode_combine joins them in order of their keys.
 //
-// Warp 8 loads (TMA; lane i box i, a page or the whole tile; with an 8-bit
-// cache also the tile's scales, as floats, a tile ahead); warps 0-7 take 16
-// keys of a tile each, with their own maximum and sum, and meet when a unit's
-// piece ends.
+// The last warp loads (TMA; lane i box i, a page or the whole tile, and with
+// an 8-bit cache its scales; a chunk of pages looked up ahead); the others
+// take strips of 16 keys in turn, each with its own maximum and sum, and meet
+// when a unit's piece ends.
 //
-// Weights are taken against a reference point 2^6 below the first maximum and
-// moved only when a score passes it by 2^14 (fp16 weights stay below 2^15, and
-// those above 2^-14 of the top keep all their bits); the division by the sum
-// of the same weights cancels it.
+// Weights are taken against a reference point 2^2 below the first maximum and
+// moved only when a score passes it by 2^8; the division by the sum of the
+// same weights cancels it.
 //
-// An 8-bit cache runs in fp16: codes are exact there.  bf16 queries are
-// brought into fp16's range by a power of two a row (exact for magnitudes
-// down to 2^-31 of the row's largest), key scales multiply the scores in
-// fp32, value scales the codes (exact while 2^-15 <= scale <= 2^7; a strip
-// of 16 keys with another one goes through fp32 into the queries' type).
+// An 8-bit cache runs in fp16, where its codes are exact.  bf16 queries are
+// brought into fp16's range by a power of two a row (exact for magnitudes down
+// to 2^-31 of the row's largest), key scales multiply the scores in fp32,
+// value scales the weights, relative to the first strip's largest scale: fp16
+// weights then keep their bits while a strip's scales lie within 2^-10 .. 2^6
+// of it; a strip with another one takes bf16 weights, whose range is fp32's.
 //
 // Values that are not finite: as in attention_tile.cu, a row whose result is
 // not finite although its sum is is computed again over its visible keys.
@@ -47,30 +55,19 @@
 namespace cmpx {
 namespace {
 
-constexpr int kKeys = 128;        // keys of a tile
-constexpr int kConsumers = 8;     // warps, 16 keys each
-constexpr int kThreads = 32 * (kConsumers + 1);
-constexpr float kBias = 6.0f, kGrow = 14.0f;
-
-template <int D, bool Q8>
-struct DecodeCfg {
-  static constexpr int ROW = Q8 ? D : 2 * D;           // bytes of a key
-  static constexpr int HALF = kKeys * ROW;             // keys, or values, of a tile
-  static constexpr int STAGES = (Q8 ? 163840 : 196608) / (2 * HALF) < 8 ? (Q8 ? 163840 : 196608) / (2 * HALF) : 8;
-  static constexpr int SCALES = Q8 ? 2 * kKeys * 4 : 0;
-  static constexpr int MERGE = 4 * 16 * D * 4;         // four warps' rows
-  static constexpr size_t SMEM = size_t(STAGES) * (2 * HALF + SCALES) + MERGE + 1024 + 2048;
-  static_assert(SMEM <= 232448, "shared memory budget");
-};
+constexpr float kBias = 2.0f, kGrow = 8.0f;
+constexpr float kNone = -3.4028234663852886e38f;  // reference point of a row without a score so far
 
 struct DecodeParams {
   SeqProblem p;
   int box_rows;     // keys of one TMA box
   int blocks;       // most blocks that share the work
   int min_tiles;    // tiles worth a block
-  float* part_o;    // [blocks][2][16][D]
-  float2* part_ml;  // [blocks][2][16]
-  int64_t* plan;    // [batch + 2]: tiles before each sequence, their number, blocks in use
+  int rows;         // of a unit: 8 or 16
+  int keys;         // of a tile
+  float* part_o;    // [blocks][2][rows][D]
+  float2* part_ml;  // [blocks][2][rows]
+  int* plan;        // [batch + 2]: tiles before each sequence, their number, blocks in use
   int* err;
 };
 
@@ -99,85 +96,125 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t cvt_e4m3x2(uint32_t two) {  // low 16 bits: two codes
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(two), __NV_E4M3);
-  return uint32_t(h.x) | uint32_t(h.y) << 16;
+// Four e4m3 codes as two fp16 pairs (exact): codes 0 and 1, codes 2 and 3.
+__device__ __forceinline__ void e4m3_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
-__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
-  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
-__device__ __forceinline__ uint32_t scaled2(uint32_t h2, float lo, float hi, __half*) {
+__device__ __forceinline__ uint32_t half2_to_bf16(uint32_t h2) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-  uint32_t r;
-  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y * hi), "f"(f.x * lo));
-  return r;
+  return pack2(f.x, f.y, (__nv_bfloat16*)nullptr);
 }
-__device__ __forceinline__ uint32_t scaled2(uint32_t h2, float lo, float hi, __nv_bfloat16*) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-  uint32_t r;
-  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y * hi), "f"(f.x * lo));
-  return r;
+// An 8 x 8 matrix of 16-bit values, turned.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
-__device__ __forceinline__ void sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory"); }
 
 // Tiles of one unit of a sequence (one even without keys: its rows are
 // written), and units of a kv head.
-__device__ __forceinline__ int unit_tiles(int len) { return max(1, (len + kKeys - 1) / kKeys); }
-__device__ __forceinline__ int row_tiles(int n, int group) { return (n * group + 15) >> 4; }
-// First tile of block c.
-__device__ __forceinline__ int64_t first_tile(int64_t c, int64_t total, int64_t used) { return c * total / used; }
+__device__ __forceinline__ int unit_tiles(const DecodeParams& a, int len) { return max(1, (len + a.keys - 1) / a.keys); }
+__device__ __forceinline__ int row_tiles(const DecodeParams& a, int n) {
+  return (n * a.p.group + a.rows - 1) / a.rows;
+}
+// First tile of block c: floor(c * total / used), c <= used <= 4096.
+__device__ __forceinline__ int first_tile(int c, int total, int used) {
+  const int q = total / used;
+  return c * q + c * (total - q * used) / used;
+}
 
 // A place in the list of tiles.
 struct Walk {
   int b, hk, rt, j;  // sequence, kv head, row tile, tile of the unit
   int nrt, nt;       // row tiles, tiles of a unit
   Seq s;
-  __device__ __forceinline__ void enter(const SeqProblem& p) {
-    s = seq_of(p, b);
-    nrt = row_tiles(s.n, p.group);
-    nt = unit_tiles(s.len);
+  __device__ __forceinline__ void enter(const DecodeParams& a) {
+    s = seq_of(a.p, b);
+    nrt = row_tiles(a, s.n);
+    nt = unit_tiles(a, s.len);
   }
-  __device__ __forceinline__ void step(const SeqProblem& p) {
+  __device__ __forceinline__ void step(const DecodeParams& a) {
     if (++j < nt) return;
     j = 0;
     if (++rt < nrt) return;
     rt = 0;
-    if (++hk < p.heads_kv) return;
+    if (++hk < a.p.heads_kv) return;
     hk = 0;
     do {
-      if (++b >= p.batch) return;  // behind the list
-      enter(p);
+      if (++b >= a.p.batch) return;  // behind the list
+      enter(a);
     } while (nrt == 0);
   }
 };
 
-// The row (16 of a unit) with index r: its token, head, and visible keys (0:
-// no such row).
+// What the loading warp tells the others of a tile; one lies beside each of
+// the ring's places.  (The others would need a Walk of their own: with it in
+// registers they spill, and with the shared memory all taken by the ring a
+// spilled register comes back from L2.)
+struct alignas(16) TileInfo {
+  int key;           // the tile's first key
+  int len;           // keys of the sequence
+  int flags;
+  int piece_key;     // first key of the piece of the unit that this block has
+  int b, hk, row0;   // sequence, kv head, first query row (token x head of the group)
+  int q0, n, k0;     // of Seq
+  int pad[2];
+};
+constexpr int kBegins = 1;   // the piece's first tile
+constexpr int kEnds = 2;     // its last one
+constexpr int kWhole = 4;    // the piece is the whole unit
+constexpr int kFirst = 8;    // the unit begins in this block
+constexpr int kLast = 16;    // the block's last tile
+
+// Query row r of a unit: its token, head, and visible keys (0: no such row).
 struct Row {
   int token, head, lim;
   bool valid;
 };
-__device__ __forceinline__ Row row_of(const SeqProblem& p, const Walk& w, int r) {
-  const int q = w.rt * 16 + r;
+__device__ __forceinline__ Row row_of(const SeqProblem& p, const TileInfo& w, int r) {
+  const int q = w.row0 + r;
   Row x;
   x.token = q / p.group;
   x.head = w.hk * p.group + q - x.token * p.group;
-  x.valid = x.token < w.s.n;
-  x.lim = x.valid ? seq_limit(p, w.s, x.token) : 0;
+  x.valid = x.token < w.n;
+  x.lim = x.valid ? seq_limit(p, Seq{w.q0, w.n, w.k0, w.len}, x.token) : 0;
   return x;
 }
 
-// Place of row r, column d among a warp pair's joined rows: rows four apart
-// share banks, so the eight a store instruction touches conflict two by two.
+// NB: 8-row column blocks of a unit.  One needs at most 128 registers a
+// thread: two blocks of eight warps an SM (registers are dealt out for four
+// warps at a time, so five-warp blocks would count as eight).  Two need 168:
+// one block of twelve.
+template <int D, bool Q8, int NB>
+struct DecodeCfg {
+  static constexpr int ROWS = 8 * NB;
+  static constexpr int PER_SM = NB == 1 ? 2 : 1;
+  static constexpr int WARPS = NB == 1 ? 7 : 11;       // consumers
+  static constexpr int THREADS = 32 * (WARPS + 1);
+  static constexpr int ROW = Q8 ? D : 2 * D;           // bytes of a key
+  static constexpr int KEYS = ROW == 256 ? 64 : 128;   // of a tile
+  static constexpr int HALF = KEYS * ROW;              // keys, or values, of a tile
+  static constexpr int RING = 196608 / PER_SM / (2 * HALF);
+  static constexpr int STAGES = RING < 8 ? RING : 8;
+  static constexpr int SCALES = Q8 ? 2 * KEYS : 0;     // a tile's e8m0 bytes
+  static constexpr int SLOTS = NB == 1 ? 3 : 2;        // sums of a piece that meet in shared memory
+  static constexpr int MERGE = SLOTS * ROWS * D * 4;
+  static constexpr size_t SMEM = size_t(STAGES) * (2 * HALF + SCALES) + MERGE + STAGES * sizeof(TileInfo) + 1024 + 256 + WARPS * ROWS * 8;
+  static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory budget");
+};
+
+// Place of row r, column d among joined rows: the eight rows a store
+// instruction touches lie on different banks.
 template <int D>
 __device__ __forceinline__ int merge_at(int r, int d) {
-  return r * D + (d ^ ((r & 3) << 3));
+  return r * D + (d ^ ((r >> 1 & 3) << 3));
 }
 
 // One row over keys [kbeg, kend) from its definition; a warp computes it.
 template <typename T, int D, bool Q8>
-__device__ __noinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk, const T* q, int kbeg, int kend,
+__device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk, const T* q, int kbeg, int kend,
                                       float m, float* merge, int r) {
   const int lane = threadIdx.x & 31;
   constexpr int NV = D / 32;
@@ -217,36 +254,39 @@ __device__ __noinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk
   for (int i = 0; i < NV; ++i) merge[merge_at<D>(r, lane + 32 * i)] = acc[i];
 }
 
-template <int FMT, int D, bool Q8>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int FMT, int D, bool Q8, int NB>
+__global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8, NB>::PER_SM)
     attention_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                             const __grid_constant__ DecodeParams a) {
-  using Cfg = DecodeCfg<D, Q8>;
+  using Cfg = DecodeCfg<D, Q8, NB>;
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
-  constexpr bool BF = FMT == 1 && !Q8;          // the products' type
-  constexpr int STAGES = Cfg::STAGES, HALF = Cfg::HALF;
-  constexpr int KSTEPS = D / 16, OT = D / 8;    // 16-wide steps of q . k, 8-wide tiles of the output
+  constexpr bool BF = FMT == 1 && !Q8;  // the products' type
+  constexpr int KEYS = Cfg::KEYS, STAGES = Cfg::STAGES, HALF = Cfg::HALF, WARPS = Cfg::WARPS, THREADS = Cfg::THREADS;
+  constexpr int DT = D / 16;            // 16-wide steps of q . k, 16-wide tiles of the output
   const SeqProblem& p = a.p;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024 - (raw & 1023)) & 1023);
   uint8_t* ring = smem;                                                        // [STAGES] keys, values
-  float* merge = reinterpret_cast<float*>(ring + size_t(STAGES) * 2 * HALF);   // [4][16][D]
-  float* scales = merge + Cfg::MERGE / 4;                                      // [STAGES][2][kKeys]
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + STAGES * (Cfg::SCALES / 4));
+  float* merge = reinterpret_cast<float*>(ring + size_t(STAGES) * 2 * HALF);   // [SLOTS][ROWS][D]
+  uint8_t* scales = reinterpret_cast<uint8_t*>(merge) + Cfg::MERGE;            // [STAGES][2][KEYS]
+  TileInfo* infos = reinterpret_cast<TileInfo*>(scales + STAGES * Cfg::SCALES);  // [STAGES]
+  uint64_t* full = reinterpret_cast<uint64_t*>(infos + STAGES);
   uint64_t* empty = full + STAGES;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + STAGES);
-  int* start = const_cast<int*>(abort_flag) + 2;                               // [4] sequence, then the place in it
-  int64_t* warp_sum = reinterpret_cast<int64_t*>(start + 4);                   // [9]
-  float2* ml = reinterpret_cast<float2*>(warp_sum + 10);                       // [8][16]
+  uint64_t* join = empty + STAGES;  // the consumers meet
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(join + 1);
+  int* start = const_cast<int*>(abort_flag) + 1;                               // [2] sequence, place in it
+  int* warp_sum = start + 2;                                                   // [WARPS + 1]
+  float2* ml = reinterpret_cast<float2*>(warp_sum + 13);                       // [WARPS][ROWS]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], Q8 ? 33 : 1);
-      mbar_init(&empty[i], kConsumers);
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], WARPS);
     }
+    mbar_init(join, WARPS);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -254,126 +294,143 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  // ---- this block's share of the tiles
-  auto tiles_of = [&](int b) -> int64_t {
-    if (b >= p.batch) return 0;
-    const Seq s = seq_of(p, b);
-    return int64_t(row_tiles(s.n, p.group)) * unit_tiles(s.len) * p.heads_kv;
-  };
-  // inclusive sum over a chunk of kThreads sequences, and the chunk's total
-  auto scan = [&](int64_t c, int64_t& all) -> int64_t {
-    int64_t inc = c;
+  // ---- this block's share of the tiles.  Sequences are counted THREADS at a
+  // time; `mine` (tiles of this thread's sequence) and `upto` (of all up to
+  // it) stay in registers where one pass holds them all.
+  int mine = 0, upto = 0;
+  auto count_pass = [&](int base) -> int {
+    const int b = base + int(threadIdx.x);
+    mine = 0;
+    if (b < p.batch) {
+      const Seq s = seq_of(p, b);
+      mine = row_tiles(a, s.n) * unit_tiles(a, s.len) * p.heads_kv;
+    }
+    upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
     }
-    if (lane == 31) warp_sum[warp] = inc;
+    if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
-    all = 0;
+    int all = 0;
 #pragma unroll
-    for (int w = 0; w <= kConsumers; ++w) {
-      if (w == warp) inc += all;
+    for (int w = 0; w <= WARPS; ++w) {
+      if (w == warp) upto += all;
       all += warp_sum[w];
     }
     __syncthreads();
-    return inc;
+    return all;
   };
-  int64_t total = 0;
-  for (int base = 0; base < p.batch; base += kThreads) {
-    const int64_t c = tiles_of(base + int(threadIdx.x));
-    int64_t all;
-    const int64_t inc = scan(c, all);
-    if (blockIdx.x == 0 && base + int(threadIdx.x) < p.batch)
-      a.plan[base + threadIdx.x] = total + inc - c;
+  int total = 0;
+  for (int base = 0; base < p.batch; base += THREADS) {
+    const int all = count_pass(base);
+    if (blockIdx.x == 0 && base + int(threadIdx.x) < p.batch) a.plan[base + threadIdx.x] = total + upto - mine;
     total += all;
   }
-  int64_t used = (total + a.min_tiles - 1) / a.min_tiles;
-  if (used > a.blocks) used = a.blocks;
+  const int used = min((total + a.min_tiles - 1) / a.min_tiles, a.blocks);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     a.plan[p.batch] = total;
     a.plan[p.batch + 1] = used;
   }
-  const int64_t c_id = blockIdx.x;
-  const int64_t lo = c_id < used ? first_tile(c_id, total, used) : 0;
-  const int64_t hi = c_id < used ? first_tile(c_id + 1, total, used) : 0;
-  int64_t before = 0;
-  for (int base = 0; lo < hi && base < p.batch; base += kThreads) {
-    const int64_t c = tiles_of(base + int(threadIdx.x));
-    int64_t all;
-    const int64_t inc = scan(c, all);
-    const int64_t rel = lo - (before + inc - c);
-    if (rel >= 0 && rel < c) {
+  const int c_id = int(blockIdx.x);
+  const int lo = c_id < used ? first_tile(c_id, total, used) : 0;
+  const int count = c_id < used ? first_tile(c_id + 1, total, used) - lo : 0;  // tiles of this block
+  for (int base = 0, before = 0; count > 0 && base < p.batch; base += THREADS) {
+    int all = total;
+    if (p.batch > THREADS) all = count_pass(base);
+    const int rel = lo - (before + upto - mine);
+    if (rel >= 0 && rel < mine) {
       start[0] = base + int(threadIdx.x);
-      *reinterpret_cast<int64_t*>(start + 2) = rel;
+      start[1] = rel;
     }
-    __syncthreads();
     before += all;
     if (lo < before) break;
   }
+  __syncthreads();
   Walk w = {};
-  if (lo < hi) {
+  if (count > 0) {
     w.b = start[0];
-    int64_t rel = *reinterpret_cast<int64_t*>(start + 2);
-    w.enter(p);
-    const int64_t per_head = int64_t(w.nrt) * w.nt;
-    w.hk = int(rel / per_head);
+    int rel = start[1];
+    w.enter(a);
+    const int per_head = w.nrt * w.nt;
+    w.hk = rel / per_head;
     rel -= w.hk * per_head;
-    w.rt = int(rel / w.nt);
-    w.j = int(rel - int64_t(w.rt) * w.nt);
+    w.rt = rel / w.nt;
+    w.j = rel - w.rt * w.nt;
   }
 
-  if (warp == kConsumers) {
+  if (warp == WARPS) {
     // ------------------------------------------------------------ loads
     if (lane == 0) {
       prefetch_tmap(&tmK);
       prefetch_tmap(&tmV);
     }
-    const int boxes_full = kKeys / a.box_rows;
-    struct Ahead {
-      int page;        // of this lane's box
-      float ks[4], vs[4];  // scales of keys 4 lane .. 4 lane + 3
+    const int boxes_full = KEYS / a.box_rows;
+    // Pages of the unit's keys, 32 at a time, a lane each: the tiles of 32
+    // pages take theirs by shuffles, and the next 32 (of this unit or the
+    // next one) are on their way meanwhile.
+    auto pages_of = [&](const Walk& x, int chunk) -> int {
+      const int at = chunk * 32 + lane;
+      return p.table != nullptr && (int64_t(at) << p.page_lg) < x.s.len ? __ldg(p.table + x.b * p.table_stride + at) : 0;
     };
-    auto look = [&](const Walk& x) -> Ahead {
-      Ahead h;
-      h.page = 0;
-      const int kv0 = x.j * kKeys;
-      if (p.table != nullptr) {
-        const int key = kv0 + lane * a.box_rows;
-        if (lane < boxes_full && key < x.s.len) h.page = __ldg(p.table + x.b * p.table_stride + key / p.page_size);
-      }
-      if constexpr (Q8) {
-        const int page = __shfl_sync(0xffffffffu, h.page, (4 * lane) / a.box_rows);
-        const bool there = page >= 0 && page < p.pages;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = kv0 + 4 * lane + i, slot = key & (p.page_size - 1);
-          h.ks[i] = h.vs[i] = 0.0f;
-          if (there && key < x.s.len) {
-            h.ks[i] = e8m0_to_float(__ldg(p.k.scale + page * p.k.s_page + x.hk * p.k.s_head + slot * p.k.s_row));
-            h.vs[i] = e8m0_to_float(__ldg(p.v.scale + page * p.v.s_page + x.hk * p.v.s_head + slot * p.v.s_row));
-          }
+    int chunk = -1, page32 = 0, next32 = 0;
+    if (count > 0) next32 = pages_of(w, (w.j * KEYS) >> p.page_lg >> 5);
+    int st = 0;
+    uint32_t phase = 1;
+    int done = 0;
+    bool ok = true;
+    for (int i = 0; i < count; ++i) {
+      const int first = (w.j * KEYS) >> p.page_lg;  // page of the tile's first key
+      if (w.j == 0 || first >> 5 != chunk) {
+        chunk = first >> 5;
+        page32 = next32;
+        if ((int64_t(chunk + 1) << p.page_lg << 5) < w.s.len) {
+          next32 = pages_of(w, chunk + 1);
+        } else if (i + w.nt - w.j < count) {
+          Walk x = w;
+          x.j = x.nt - 1;
+          x.step(a);
+          next32 = pages_of(x, 0);
         }
       }
-      return h;
-    };
-    Ahead next = {};
-    if (lo < hi) next = look(w);
-    int64_t done = 0;
-    bool ok = true;
-    for (int64_t i = lo; i < hi; ++i) {
-      const Ahead now = next;
-      const int hk = w.hk, kv0 = w.j * kKeys, k0 = w.s.k0;
+      const int now = __shfl_sync(0xffffffffu, page32, first + lane);  // (modulo 32)
+      const int hk = w.hk, kv0 = w.j * KEYS, k0 = w.s.k0;
+      TileInfo info;
+      info.key = kv0;
+      info.len = w.s.len;
+      info.flags = (i == 0 || w.j == 0 ? kBegins : 0) | (i + 1 == count || w.j + 1 == w.nt ? kEnds : 0) |
+                   (i >= w.j ? kFirst : 0) | (i >= w.j && w.j + 1 == w.nt ? kWhole : 0) | (i + 1 == count ? kLast : 0);
+      info.piece_key = i >= w.j ? 0 : (w.j - i) * KEYS;
+      info.b = w.b;
+      info.hk = hk;
+      info.row0 = w.rt * a.rows;
+      info.q0 = w.s.q0;
+      info.n = w.s.n;
+      info.k0 = k0;
       const int boxes = min(boxes_full, (w.s.len - kv0 + a.box_rows - 1) / a.box_rows);
-      w.step(p);
-      if (i + 1 < hi) next = look(w);
-      const int st = int((i - lo) % STAGES);
-      if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], uint32_t(((i - lo) / STAGES) & 1) ^ 1u, abort_flag))) {
+      if (i + 1 < count) w.step(a);
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], phase, abort_flag))) {
         if (lane == 0) rec_err(a.err, abort_flag, kDevTimeoutEmpty);
         ok = false;
         break;
       }
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], uint32_t(max(boxes, 0) * a.box_rows * Cfg::ROW * 2));
+      // scales of pages that are none: zeros, as TMA gives for their codes
+      const bool there = lane < boxes && now >= 0 && now < p.pages;
+      uint32_t bytes = uint32_t(max(boxes, 0) * a.box_rows * Cfg::ROW * 2);
+      if constexpr (Q8) {
+        if (lane < boxes && !there)
+          for (int k = 0; k < a.box_rows; k += 4)
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+              *reinterpret_cast<uint32_t*>(scales + st * Cfg::SCALES + v * KEYS + lane * a.box_rows + k) = 0u;
+        bytes += uint32_t(__popc(__ballot_sync(0xffffffffu, there)) * a.box_rows * 2);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        infos[st] = info;
+        mbar_arrive_expect_tx(&full[st], bytes);
+      }
       __syncwarp();
       if (lane < boxes) {
         uint8_t* kd = ring + size_t(st) * 2 * HALF;
@@ -383,350 +440,404 @@ __global__ void __launch_bounds__(kThreads, 1)
           const CUtensorMap* m = v ? &tmV : &tmK;
           uint8_t* dst = kd + v * HALF;
           if constexpr (Cfg::ROW <= 128) {
-            tma_load_4d(dst + lane * a.box_rows * Cfg::ROW, m, &full[st], 0, row, hk, now.page);
+            tma_load_4d(dst + lane * a.box_rows * Cfg::ROW, m, &full[st], 0, row, hk, now);
           } else {
 #pragma unroll
             for (int c = 0; c < 2; ++c)
-              tma_load_4d(dst + c * (HALF / 2) + lane * a.box_rows * 128, m, &full[st], c * 64, row, hk, now.page);
+              tma_load_4d(dst + c * (HALF / 2) + lane * a.box_rows * 128, m, &full[st], c * 64, row, hk, now);
+          }
+          if constexpr (Q8) {
+            const SeqKV& kv = v ? p.v : p.k;
+            if (there)
+              bulk_load(scales + st * Cfg::SCALES + v * KEYS + lane * a.box_rows,
+                        kv.scale + now * kv.s_page + hk * kv.s_head + row, uint32_t(a.box_rows), &full[st]);
           }
         }
       }
-      if constexpr (Q8) {
-        float* sc = scales + st * 2 * kKeys;
-        *reinterpret_cast<float4*>(sc + 4 * lane) = make_float4(now.ks[0], now.ks[1], now.ks[2], now.ks[3]);
-        *reinterpret_cast<float4*>(sc + kKeys + 4 * lane) = make_float4(now.vs[0], now.vs[1], now.vs[2], now.vs[3]);
-        mbar_arrive(&full[st]);
-      }
       ++done;
+      if (++st == STAGES) {
+        st = 0;
+        phase ^= 1u;
+      }
     }
     if (!ok && lane == 0) {
       // let the copies in flight land before the block exits (bounded waits)
       volatile int never = 0;
-      for (int64_t i = done > STAGES ? done - STAGES : 0; i < done; ++i)
+      for (int i = done > STAGES ? done - STAGES : 0; i < done; ++i)
         mbar_wait(&full[i % STAGES], uint32_t((i / STAGES) & 1), &never);
     }
   } else {
     // ------------------------------------------------------------ products and softmax
     const int g = lane >> 2, t = lane & 3;
-    const int key_w = warp * 16;  // this warp's keys of a tile
-    uint32_t qf[KSTEPS][4];
-    float o[OT][4];
-    float m[2], l[2], qs[2];  // rows g and g + 8: reference point, sum (this lane's keys), score factor
-    int lim[2] = {0, 0};
-    bool fresh = true, ok = true;
-    const int mi = lane >> 3, mr = lane & 7;
-    for (int64_t i = lo; i < hi; ++i) {
-      if (fresh) {
-        fresh = false;
+    // 16-byte unit u of strip row r lies at r * row bytes + ((u ^ swizzle) << 4);
+    // this lane's row and unit of a 16 x 2-unit ldmatrix, whose four parts are
+    // (rows 0-7, unit 0), (rows 8-15, unit 0), (rows 0-7, unit 1), (rows 8-15, unit 1)
+    uint32_t lane_at;
+    {
+      const int row = (lane >> 3 & 1) * 8 + (lane & 7), unit = lane >> 4;
+      constexpr int PITCH = Cfg::ROW < 128 ? 64 : 128;
+      lane_at = row * PITCH + ((unit ^ (PITCH == 64 ? row >> 1 & 3 : row & 7)) << 4);
+    }
+    // units 2 i and 2 i + 1 of the strip at `base`
+    auto ldsm_at = [&](uint32_t base, int i) -> uint32_t {
+      if constexpr (Cfg::ROW == 256) return (base ^ ((2 * i & 7) << 4)) + (i >> 2) * (HALF / 2);
+      else return base ^ (2 * i << 4);
+    };
+    constexpr int PITCH = Cfg::ROW < 128 ? 64 : 128;
+    uint32_t qf[DT][NB][2];               // Q^T: row g of block nb
+    float o[DT][NB][4];                   // O^T: two columns, rows 2t and 2t + 1
+    float m[NB][2], l[NB][2], qs[NB][2];  // rows 2t, 2t + 1: reference point, sum (this lane's keys), score factor
+    int lim[NB][2];
+    int lim_min = 0;                      // of all rows
+    float v_ref = 0.0f;                   // 8-bit: 1 / the scale that value scales are relative to (0: none yet)
+    int strip = warp;                     // the next of this warp's strips, counted from the tile's first
+    int st = 0, flags = count > 0 ? 0 : kLast;
+    uint32_t phase = 0, join_phase = 0;
+    bool ok = true;
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(join);
+      ok = __all_sync(0xffffffffu, mbar_wait(join, join_phase, abort_flag)) && ok;
+      join_phase ^= 1u;
+    };
+    while (ok && !(flags & kLast)) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, abort_flag))) {
+        ok = false;
+        break;
+      }
+      const TileInfo& info = infos[st];
+      flags = info.flags;
+      if (flags & kBegins) {
+        v_ref = 0.0f;
+        lim_min = info.len;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Row r = row_of(p, w, g + 8 * h);
-          lim[h] = r.valid ? r.lim : w.s.len;  // rows of nothing hide nothing
-          m[h] = -INFINITY;
-          l[h] = 0.0f;
-          qs[h] = p.scale_log2;
-          const T* q = static_cast<const T*>(p.Q) + int64_t(w.s.q0 + r.token) * p.q_token + r.head * p.q_head;
+        for (int nb = 0; nb < NB; ++nb) {
+          const Row r = row_of(p, info, 8 * nb + g);
+          const T* q = static_cast<const T*>(p.Q) + int64_t(info.q0 + r.token) * p.q_token + r.head * p.q_head;
+          float up = 1.0f;
           if constexpr (!Q8) {
 #pragma unroll
-            for (int k = 0; k < KSTEPS; ++k) {
-              qf[k][h] = r.valid ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t) : 0u;
-              qf[k][2 + h] = r.valid ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 + 2 * t) : 0u;
-            }
+            for (int k = 0; k < DT; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                qf[k][nb][e] = r.valid ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 8 * e + 2 * t) : 0u;
           } else {
             // the codes of a key arrive four consecutive ones a lane, so the
             // products' inner index is dealt out the same way
-            uint2 x[KSTEPS];
 #pragma unroll
-            for (int k = 0; k < KSTEPS; ++k)
-              x[k] = r.valid ? *reinterpret_cast<const uint2*>(q + 16 * k + 4 * t) : make_uint2(0u, 0u);
+            for (int k = 0; k < DT; ++k) {
+              const uint2 x = r.valid ? *reinterpret_cast<const uint2*>(q + 16 * k + 4 * t) : make_uint2(0u, 0u);
+              qf[k][nb][0] = x.x;
+              qf[k][nb][1] = x.y;
+            }
             if constexpr (FMT == 1) {
               uint32_t top = 0;  // largest magnitude, as bf16 bits
 #pragma unroll
-              for (int k = 0; k < KSTEPS; ++k) {
-                top = max(top, max(x[k].x & 0x7fffu, x[k].x >> 16 & 0x7fffu));
-                top = max(top, max(x[k].y & 0x7fffu, x[k].y >> 16 & 0x7fffu));
-              }
+              for (int k = 0; k < DT; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  top = max(top, max(qf[k][nb][e] & 0x7fffu, qf[k][nb][e] >> 16 & 0x7fffu));
               top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
               top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
               // the row times 2^(14 - k), 2^k <= top < 2^(k + 1): below 2^15
-              const int e = int(top >> 7);
-              const bool plain = e == 0 || e == 255;
-              const float down = plain ? 1.0f : __uint_as_float(uint32_t(min(max(127 + 14 + 127 - e, 1), 254)) << 23);
-              const float up = plain ? 1.0f : 1.0f / down;
-              qs[h] = p.scale_log2 * up;
+              const int e2 = int(top >> 7);
+              const bool plain = e2 == 0 || e2 == 255;
+              const float down = plain ? 1.0f : __uint_as_float(uint32_t(min(268 - e2, 254)) << 23);
+              up = 1.0f / down;
 #pragma unroll
-              for (int k = 0; k < KSTEPS; ++k) {
-                x[k].x = pack2(__uint_as_float(x[k].x << 16) * down, __uint_as_float(x[k].x & 0xffff0000u) * down,
-                               (__half*)nullptr);
-                x[k].y = pack2(__uint_as_float(x[k].y << 16) * down, __uint_as_float(x[k].y & 0xffff0000u) * down,
-                               (__half*)nullptr);
-              }
-            }
+              for (int k = 0; k < DT; ++k)
 #pragma unroll
-            for (int k = 0; k < KSTEPS; ++k) {
-              qf[k][h] = x[k].x;
-              qf[k][2 + h] = x[k].y;
+                for (int e = 0; e < 2; ++e)
+                  qf[k][nb][e] = pack2(__uint_as_float(qf[k][nb][e] << 16) * down,
+                                       __uint_as_float(qf[k][nb][e] & 0xffff0000u) * down, (__half*)nullptr);
             }
+          }
+          const int keys = r.valid ? r.lim : info.len;  // rows of nothing hide nothing
+          lim_min = min(lim_min, __reduce_min_sync(0xffffffffu, keys));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            qs[nb][e] = p.scale_log2 * __shfl_sync(0xffffffffu, up, 4 * (2 * t + e));
+            lim[nb][e] = __shfl_sync(0xffffffffu, keys, 4 * (2 * t + e));
+            m[nb][e] = kNone;
+            l[nb][e] = 0.0f;
           }
         }
 #pragma unroll
-        for (int k = 0; k < OT; ++k)
+        for (int k = 0; k < DT; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[k][e] = 0.0f;
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][nb][e] = 0.0f;
       }
-      const int st = int((i - lo) % STAGES);
-      if (ok && !__all_sync(0xffffffffu, mbar_wait(&full[st], uint32_t(((i - lo) / STAGES) & 1), abort_flag))) {
-        if (lane == 0) rec_err(a.err, abort_flag, kDevTimeoutFull);
-        ok = false;
-      }
-      const int kv0 = w.j * kKeys + key_w;
-      if (ok && kv0 < w.s.len) {
-        const uint32_t kbase = smem_u32(ring + size_t(st) * 2 * HALF), vbase = kbase + HALF;
-        // address of 16-byte unit u of row r (128- or 64-byte swizzled rows)
-        auto unit_at = [&](uint32_t base, int r, int u) -> uint32_t {
-          if constexpr (Cfg::ROW == 256) return base + (u >> 3) * (HALF / 2) + r * 128 + (((u & 7) ^ (r & 7)) << 4);
-          else if constexpr (Cfg::ROW == 128) return base + r * 128 + ((u ^ (r & 7)) << 4);
-          else return base + r * 64 + ((u ^ (r >> 1 & 3)) << 4);
-        };
-        // ---- scores of 16 rows x 16 keys: two tiles of 8 keys
-        float s[2][4];
+#pragma unroll 1
+      for (; strip < KEYS / 16; strip += WARPS) {
+        const int kv0 = info.key + strip * 16;
+        const int tail = info.len - kv0;  // keys of the strip
+        if (tail <= 0) continue;
+        const uint32_t kbase = smem_u32(ring) + st * 2 * HALF + strip * 16 * PITCH + lane_at, vbase = kbase + HALF;
+        // ---- scores: keys g and g + 8, rows 2t and 2t + 1; even and odd
+        // steps in chains of their own
+        float s2[2][NB][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s2[c][nb][e] = 0.0f;
         if constexpr (!Q8) {
 #pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) {
+          for (int k = 0; k < DT; ++k) {
             uint32_t b[4];
-            ldsm_x4(b, unit_at(kbase, key_w + (mi >> 1) * 8 + mr, 2 * k + (mi & 1)));
-            mma16<BF>(s[0], qf[k], b[0], b[1]);
-            mma16<BF>(s[1], qf[k], b[2], b[3]);
+            ldsm_x4(b, ldsm_at(kbase, k));
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) mma16<BF>(s2[k & 1][nb], b, qf[k][nb][0], qf[k][nb][1]);
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < KSTEPS; k += 2) {
-            uint32_t b[4];
-            ldsm_x4(b, unit_at(kbase, key_w + (mi >> 1) * 8 + mr, k + (mi & 1)));
+          for (int k = 0; k < DT; k += 2) {
+            uint32_t b[4];  // keys 0-7 and 8-15 of units k and k + 1
+            ldsm_x4(b, ldsm_at(kbase, k / 2));
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int u = 0; u < 2; ++u) {
+              uint32_t f[4];
+              e4m3_to_half(b[2 * u], f[0], f[2]);
+              e4m3_to_half(b[2 * u + 1], f[1], f[3]);
 #pragma unroll
-              for (int kk = 0; kk < 2; ++kk)
-                mma16<false>(s[n], qf[k + kk], cvt_e4m3x2(b[2 * n + kk] & 0xffffu), cvt_e4m3x2(b[2 * n + kk] >> 16));
+              for (int nb = 0; nb < NB; ++nb) mma16<false>(s2[u][nb], f, qf[k + u][nb][0], qf[k + u][nb][1]);
+            }
           }
         }
-        // ---- scores in log2 units; hidden ones -inf
-        const float* sc = scales + st * 2 * kKeys + key_w;
+        const uint8_t* sc = scales + st * Cfg::SCALES + strip * 16 + g;
+        float ks[2] = {1.0f, 1.0f};
+        if constexpr (Q8) {
+          ks[0] = e8m0_to_float(sc[0]);
+          ks[1] = e8m0_to_float(sc[8]);
+        }
+        // in log2 units; hidden scores -inf
+        float s[NB][4];
+        bool grew = false;
+        const bool cut = kv0 + 16 > lim_min;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          float2 kf = make_float2(1.0f, 1.0f);
-          if constexpr (Q8) kf = *reinterpret_cast<const float2*>(sc + 8 * n + 2 * t);
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[n][e] *= qs[e >> 1];
-            if constexpr (Q8) s[n][e] *= (e & 1) ? kf.y : kf.x;
+            s[nb][e] = (s2[0][nb][e] + s2[1][nb][e]) * qs[nb][e & 1];
+            if constexpr (Q8) s[nb][e] *= ks[e >> 1];
           }
-        }
-        const int edge = min(lim[0], lim[1]) - kv0;
-        const bool cut = __any_sync(0xffffffffu, edge < 16);
-        if (cut) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
+          if (cut) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (kv0 + 8 * n + 2 * t + (e & 1) >= lim[e >> 1]) s[n][e] = -INFINITY;
-        }
-        float mx[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-        const bool grew = mx[0] > m[0] + kGrow || mx[1] > m[1] + kGrow;
-        if (__any_sync(0xffffffffu, grew)) {
-          float alpha[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            const float m_new = mx[h] > m[h] + kGrow ? mx[h] - kBias : m[h];
-            alpha[h] = m_new == m[h] ? 1.0f : ex2_approx(m[h] - m_new);
-            m[h] = m_new;
-            l[h] *= alpha[h];
+              if (kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]) s[nb][e] = -INFINITY;
           }
-#pragma unroll
-          for (int k = 0; k < OT; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[k][e] *= alpha[e >> 1];
+          grew = grew || fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kGrow || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kGrow;
         }
+        if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float mu = m[h] == -INFINITY ? 0.0f : m[h];
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float wgt = ex2_approx(s[n][2 * h + e] - mu);
-              s[n][2 * h + e] = wgt;
-              l[h] += wgt;
+              float mx = fmaxf(s[nb][e], s[nb][e + 2]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+              const bool up = mx > m[nb][e] + kGrow;
+              const float m_new = up ? mx - kBias : m[nb][e];
+              const float alpha = up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
+              m[nb][e] = m_new;
+              l[nb][e] *= alpha;
+#pragma unroll
+              for (int k = 0; k < DT; ++k) {
+                o[k][nb][e] *= alpha;
+                o[k][nb][e + 2] *= alpha;
+              }
             }
         }
-        // ---- O += P V
-        const int tail = w.s.len - kv0;  // keys of the strip
-        // value rows behind the last key may hold anything: lanes clear theirs
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (tail < 16) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            keep[h] = (8 * h + 2 * t < tail ? 0xffffu : 0u) | (8 * h + 2 * t + 1 < tail ? 0xffff0000u : 0u);
-        }
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[nb][e] = ex2_approx(s[nb][e] - m[nb][e & 1]);
+            l[nb][e & 1] += s[nb][e];
+          }
+        // ---- O^T += V^T P^T.  Value rows behind the last key may hold
+        // anything: their elements are cleared
+        auto keep = [&](int h) -> uint32_t {
+          return (8 * h + 2 * t < tail ? 0xffffu : 0u) | (8 * h + 2 * t + 1 < tail ? 0xffff0000u : 0u);
+        };
         if constexpr (!Q8) {
-          const uint32_t pf[4] = {pack2(s[0][0], s[0][1], (T*)nullptr), pack2(s[0][2], s[0][3], (T*)nullptr),
-                                  pack2(s[1][0], s[1][1], (T*)nullptr), pack2(s[1][2], s[1][3], (T*)nullptr)};
+          auto add = [&](auto clear) {
+            uint32_t pf[NB][2];
 #pragma unroll
-          for (int k = 0; k < OT; k += 2) {
-            uint32_t b[4];
-            ldsm_x4_t(b, unit_at(vbase, key_w + (mi & 1) * 8 + mr, k + (mi >> 1)));
-            mma16<BF>(o[k], pf, b[0] & keep[0], b[1] & keep[1]);
-            mma16<BF>(o[k + 1], pf, b[2] & keep[0], b[3] & keep[1]);
-          }
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (T*)nullptr));
+#pragma unroll
+            for (int k = 0; k < DT; ++k) {
+              uint32_t b[4];
+              ldsm_x4_t(b, ldsm_at(vbase, k));
+              uint32_t f[4] = {b[0], b[2], b[1], b[3]};
+              if constexpr (decltype(clear)::value) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] &= keep(e >> 1);
+              }
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma16<BF>(o[k][nb], f, pf[nb][0], pf[nb][1]);
+            }
+          };
+          if (tail < 16) add(std::true_type());
+          else add(std::false_type());
         } else {
-          const float2 v0 = *reinterpret_cast<const float2*>(sc + kKeys + 2 * t);
-          const float2 v1 = *reinterpret_cast<const float2*>(sc + kKeys + 8 + 2 * t);
-          // (0: a key that is not there)
-          auto fits = [](float x) -> bool { return x == 0.0f || (x >= 0x1p-15f && x <= 0x1p7f); };
-          const bool small = fits(v0.x) && fits(v0.y) && fits(v1.x) && fits(v1.y);
-          if (__all_sync(0xffffffffu, small)) {
-            const uint32_t pf[4] = {
-                pack2(s[0][0], s[0][1], (__half*)nullptr), pack2(s[0][2], s[0][3], (__half*)nullptr),
-                pack2(s[1][0], s[1][1], (__half*)nullptr), pack2(s[1][2], s[1][3], (__half*)nullptr)};
-            const uint32_t sv[2] = {pack2(v0.x, v0.y, (__half*)nullptr), pack2(v1.x, v1.y, (__half*)nullptr)};
+          float vs[2];
+          vs[0] = e8m0_to_float(sc[KEYS]);
+          vs[1] = e8m0_to_float(sc[KEYS + 8]);
+          if (v_ref == 0.0f) {
+            float top = fmaxf(g < tail ? vs[0] : 0.0f, g + 8 < tail ? vs[1] : 0.0f);  // drops a NaN
 #pragma unroll
-            for (int k = 0; k < KSTEPS; k += 2) {
-              uint32_t b[4];
-              ldsm_x4_t(b, unit_at(vbase, key_w + (mi & 1) * 8 + mr, k + (mi >> 1)));
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int odd = 0; odd < 2; ++odd) {
-                  const uint32_t c0 = __byte_perm(b[2 * u], 0, odd ? 0x4431 : 0x4420);
-                  const uint32_t c1 = __byte_perm(b[2 * u + 1], 0, odd ? 0x4431 : 0x4420);
-                  mma16<false>(o[2 * (k + u) + odd], pf, mul_h2(cvt_e4m3x2(c0), sv[0]) & keep[0],
-                               mul_h2(cvt_e4m3x2(c1), sv[1]) & keep[1]);
-                }
-            }
-          } else {
-            const uint32_t pf[4] = {pack2(s[0][0], s[0][1], (T*)nullptr), pack2(s[0][2], s[0][3], (T*)nullptr),
-                                    pack2(s[1][0], s[1][1], (T*)nullptr), pack2(s[1][2], s[1][3], (T*)nullptr)};
-#pragma unroll
-            for (int k = 0; k < KSTEPS; k += 2) {
-              uint32_t b[4];
-              ldsm_x4_t(b, unit_at(vbase, key_w + (mi & 1) * 8 + mr, k + (mi >> 1)));
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int odd = 0; odd < 2; ++odd) {
-                  const uint32_t c0 = __byte_perm(b[2 * u], 0, odd ? 0x4431 : 0x4420);
-                  const uint32_t c1 = __byte_perm(b[2 * u + 1], 0, odd ? 0x4431 : 0x4420);
-                  mma16<FMT == 1>(o[2 * (k + u) + odd], pf, scaled2(cvt_e4m3x2(c0), v0.x, v0.y, (T*)nullptr) & keep[0],
-                                  scaled2(cvt_e4m3x2(c1), v1.x, v1.y, (T*)nullptr) & keep[1]);
-                }
-            }
+            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            v_ref = 1.0f / fminf(fmaxf(top, 0x1p-126f), 0x1p126f);
           }
+          bool near = true;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            vs[h] = g + 8 * h < tail ? vs[h] * v_ref : 1.0f;
+            near = near && vs[h] >= 0x1p-10f && vs[h] <= 0x1p6f;
+          }
+          near = __all_sync(0xffffffffu, near);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // (a hidden key's scale may be a NaN, which is not near)
+              s[nb][e] = !near && s[nb][e] == 0.0f ? 0.0f : s[nb][e] * vs[e >> 1];
+          auto add = [&](auto half_type, auto clear) {
+            using P = decltype(half_type);
+            constexpr bool kBf = std::is_same<P, __nv_bfloat16>::value;
+            uint32_t pf[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (P*)nullptr));
+#pragma unroll
+            for (int k = 0; k < DT; k += 2) {
+              uint32_t b[4];  // units k and k + 1, each keys 0-7 and 8-15
+              ldsm_x4_t(b, ldsm_at(vbase, k / 2));
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                // codes of two keys: even columns (rows 0-7 of the 16-wide
+                // side) together, and odd ones
+                uint32_t f[4];
+                e4m3_to_half(__byte_perm(b[2 * u], 0, 0x3120), f[0], f[1]);
+                e4m3_to_half(__byte_perm(b[2 * u + 1], 0, 0x3120), f[2], f[3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if constexpr (kBf) f[e] = half2_to_bf16(f[e]);
+                  if constexpr (decltype(clear)::value) f[e] &= keep(e >> 1);
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) mma16<kBf>(o[k + u][nb], f, pf[nb][0], pf[nb][1]);
+              }
+            }
+          };
+          if (!near) add(__nv_bfloat16(), std::true_type());
+          else if (tail < 16) add(__half(), std::true_type());
+          else add(__half(), std::false_type());
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
+      strip -= KEYS / 16;
 
-      if (w.j + 1 == w.nt || i + 1 == hi) {
-        // ---- the piece ends: join the eight warps, two rows a lane group
-        const int64_t unit0 = i - w.j;  // the unit's first tile
-        const bool whole = unit0 >= lo && w.j + 1 == w.nt;
+      if (flags & kEnds) {
+        // ---- join the warps
+        constexpr int ROWS = Cfg::ROWS, SLOTS = Cfg::SLOTS;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-          if (t == 0) ml[warp * 16 + g + 8 * h] = make_float2(m[h], l[h]);
-        }
-        sync_consumers();
-        float mt[2], lt[2], f[2];
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mt[h] = -INFINITY;
-          lt[h] = 0.0f;
+          for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int x = 0; x < kConsumers; ++x) {
-            const float2 y = ml[x * 16 + g + 8 * h];
-            if (y.y != 0.0f) mt[h] = fmaxf(mt[h], y.x);
+            for (int x = 4; x < 32; x <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], x);
+            if (g == 0) ml[warp * ROWS + 8 * nb + 2 * t + e] = make_float2(m[nb][e], l[nb][e]);
+          }
+        meet();
+        auto total_of = [&](int r) -> float2 {
+          float mt = kNone, lt = 0.0f;
+#pragma unroll
+          for (int x = 0; x < WARPS; ++x) {
+            const float2 y = ml[x * ROWS + r];
+            if (y.y != 0.0f) mt = fmaxf(mt, y.x);
           }
 #pragma unroll
-          for (int x = 0; x < kConsumers; ++x) {
-            const float2 y = ml[x * 16 + g + 8 * h];
-            if (y.y != 0.0f) lt[h] += y.y * ex2_approx(y.x - mt[h]);
+          for (int x = 0; x < WARPS; ++x) {
+            const float2 y = ml[x * ROWS + r];
+            if (y.y != 0.0f) lt += y.y * ex2_approx(y.x - mt);
           }
-          f[h] = l[h] == 0.0f ? 0.0f : ex2_approx(m[h] - mt[h]);
-        }
-        // column of element e of output tile k
-        auto col = [&](int k, int e) -> int { return Q8 ? 16 * (k >> 1) + (k & 1) + 4 * t + 2 * e : 8 * k + 2 * t + e; };
-        // warps 4-7 hand their rows to warps 0-3, which add theirs: four sums
-        float* mine = merge + (warp & 3) * 16 * D;
+          return make_float2(mt, lt);
+        };
+        const float v_up = Q8 && v_ref != 0.0f ? 1.0f / v_ref : 1.0f;
+        // the warps add their rows, SLOTS at a time, always in the same order
+        float* mine = merge + (warp % SLOTS) * ROWS * D;
+#pragma unroll 1
+        for (int pass = 0; pass < (WARPS + SLOTS - 1) / SLOTS; ++pass) {
+          if (warp / SLOTS == pass) {
 #pragma unroll
-        for (int pass = 0; pass < 2; ++pass) {
-          if ((warp >= 4) == (pass == 0)) {
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int k = 0; k < OT; ++k)
+              for (int e = 0; e < 2; ++e) {
+                const int r = 8 * nb + 2 * t + e;
+                const float f = ex2_approx(m[nb][e] - total_of(r).x) * v_up;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float* at = mine + merge_at<D>(g + 8 * (e >> 1), col(k, e & 1));
-                // a warp that saw no key leaves zeros, whatever 0 * its sums is
-                const float x = l[e >> 1] == 0.0f ? 0.0f : o[k][e] * f[e >> 1];
-                *at = pass == 0 ? x : *at + x;
+                for (int k = 0; k < DT; ++k)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    float* at = mine + merge_at<D>(r, 16 * k + (Q8 ? 2 * g + h : g + 8 * h));
+                    // a warp that saw no key leaves zeros, whatever 0 * its sums is
+                    const float x = l[nb][e] == 0.0f ? 0.0f : o[k][nb][e + 2 * h] * f;
+                    *at = pass == 0 ? x : *at + x;
+                  }
               }
           }
-          sync_consumers();
+          meet();
         }
-        // ---- write out: warp x the rows x and x + 8
+        // ---- write out, a warp a row
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int r = warp + 8 * h;
-          const Row row = row_of(p, w, r);
-          float mr2 = -INFINITY, lr = 0.0f;
-          for (int x = 0; x < kConsumers; ++x) {
-            const float2 y = ml[x * 16 + r];
-            if (y.y != 0.0f) mr2 = fmaxf(mr2, y.x);
-          }
-          for (int x = 0; x < kConsumers; ++x) {
-            const float2 y = ml[x * 16 + r];
-            if (y.y != 0.0f) lr += y.y * ex2_approx(y.x - mr2);
-          }
+        for (int r = warp; r < ROWS; r += WARPS) {
+          const Row row = row_of(p, info, r);
+          const float2 tot = total_of(r);
           bool bad = false;
+#pragma unroll
           for (int d = lane; d < D; d += 32) {
             float* at = merge + merge_at<D>(r, d);
-            const float x = (at[0] + at[16 * D]) + (at[32 * D] + at[48 * D]);
+            float x = 0.0f;
+#pragma unroll
+            for (int y = 0; y < SLOTS; ++y) x += at[y * ROWS * D];
             bad = bad || (__float_as_uint(x) & 0x7fffffffu) >= 0x7f800000u;
             at[0] = x;
           }
-          bad = __any_sync(0xffffffffu, bad) && row.valid && lr > 0.0f && lr <= 3.4028234663852886e38f;
-          const T* q = static_cast<const T*>(p.Q) + int64_t(w.s.q0 + row.token) * p.q_token + row.head * p.q_head;
-          const int first = int((whole || unit0 >= lo) ? 0 : lo - unit0) * kKeys;
+          bad = __any_sync(0xffffffffu, bad) && row.valid && tot.y > 0.0f && tot.y <= 3.4028234663852886e38f;
+          const T* q = static_cast<const T*>(p.Q) + int64_t(info.q0 + row.token) * p.q_token + row.head * p.q_head;
           if (ok && bad)
-            redo_row<T, D, Q8>(p, w.b, w.s.k0, w.hk, q, first, min(row.lim, (w.j + 1) * kKeys), mr2, merge, r);
+            redo_row<T, D, Q8>(p, info.b, info.k0, info.hk, q, info.piece_key, min(row.lim, info.key + KEYS), tot.x,
+                               merge, r);
           __syncwarp();
           if (!ok || !row.valid) continue;
-          if (whole) {
-            const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
-            T* out = static_cast<T*>(p.O) + int64_t(w.s.q0 + row.token) * p.o_token + row.head * p.o_head;
-            for (int d = lane; d < D; d += 32) stf(out + d, lr == 0.0f ? 0.0f : merge[merge_at<D>(r, d)] * inv);
+          if (flags & kWhole) {
+            const float inv = tot.y == 0.0f ? 0.0f : 1.0f / tot.y;
+            T* out = static_cast<T*>(p.O) + int64_t(info.q0 + row.token) * p.o_token + row.head * p.o_head;
+            for (int d = lane; d < D; d += 32) stf(out + d, tot.y == 0.0f ? 0.0f : merge[merge_at<D>(r, d)] * inv);
           } else {
             // a piece of a unit that began in an earlier block goes to the
             // first place, one that goes on in the next block to the second
-            const int64_t at = (c_id * 2 + (unit0 >= lo ? 1 : 0)) * 16 + r;
-            if (lane == 0) a.part_ml[at] = make_float2(mr2, lr);
+            const int64_t at = (int64_t(blockIdx.x) * 2 + (flags & kFirst ? 1 : 0)) * ROWS + r;
+            if (lane == 0) a.part_ml[at] = tot;
             for (int d = lane; d < D; d += 32) a.part_o[at * D + d] = merge[merge_at<D>(r, d)];
           }
         }
-        sync_consumers();
-        fresh = true;
+        meet();  // the merge area is free again
       }
-      w.step(p);  // a warp that gave up keeps walking: the others meet it where pieces end
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      if (++st == STAGES) {
+        st = 0;
+        phase ^= 1u;
+      }
     }
+    if (!ok && lane == 0) rec_err(a.err, abort_flag, kDevTimeoutFull);
   }
 }
 
@@ -764,16 +875,16 @@ __global__ void __launch_bounds__(128) attention_decode_combine(const DecodePara
   const Seq s = seq_of(p, b);
   if (t < s.q0 || t >= s.q0 + s.n) return;
   const int hk = h / p.group, q = (t - s.q0) * p.group + h - hk * p.group;
-  const int nt = unit_tiles(s.len), nrt = row_tiles(s.n, p.group);
-  const int64_t total = a.plan[p.batch], used = a.plan[p.batch + 1];
-  const int64_t first = a.plan[b] + (int64_t(hk) * nrt + (q >> 4)) * nt;
+  const int nt = unit_tiles(a, s.len), nrt = row_tiles(a, s.n);
+  const int total = a.plan[p.batch], used = a.plan[p.batch + 1];
+  const int first = a.plan[b] + (hk * nrt + q / a.rows) * nt;
   // block that holds a tile: the last c with c * total / used <= tile
-  const int64_t c0 = min(((first + 1) * used - 1) / total, used - 1);
-  const int64_t c1 = min(((first + nt) * used - 1) / total, used - 1);
+  const int c0 = min(int((int64_t(first + 1) * used - 1) / total), used - 1);
+  const int c1 = min(int((int64_t(first + nt) * used - 1) / total), used - 1);
   if (c0 >= c1) return;  // whole in one block: written there
-  auto at = [&](int64_t c) -> int64_t { return (c * 2 + (first_tile(c, total, used) <= first ? 1 : 0)) * 16 + (q & 15); };
+  auto at = [&](int c) -> int64_t { return (int64_t(c) * 2 + (first_tile(c, total, used) <= first ? 1 : 0)) * a.rows + q % a.rows; };
   float m = -INFINITY;
-  for (int64_t c = c0 + lane; c <= c1; c += 32) {
+  for (int c = c0 + lane; c <= c1; c += 32) {
     const float2 ml = a.part_ml[at(c)];
     if (ml.y != 0.0f) m = fmaxf(m, ml.x);
   }
@@ -782,7 +893,7 @@ __global__ void __launch_bounds__(128) attention_decode_combine(const DecodePara
   float l = 0.0f, o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.0f;
-  for (int64_t c = c0; c <= c1; ++c) {
+  for (int c = c0; c <= c1; ++c) {
     const int64_t x = at(c);
     const float2 ml = a.part_ml[x];
     if (ml.y == 0.0f) continue;
@@ -797,19 +908,26 @@ __global__ void __launch_bounds__(128) attention_decode_combine(const DecodePara
 }
 
 // ------------------------------------------------------------------ host
-int64_t decode_blocks(const DeviceInfo& dev) { return dev.num_sms; }
+int decode_keys(const SeqProblem& p, bool q8) {
+  return p.d == 64 ? (q8 ? DecodeCfg<64, true, 1>::KEYS : DecodeCfg<64, false, 1>::KEYS)
+                   : (q8 ? DecodeCfg<128, true, 1>::KEYS : DecodeCfg<128, false, 1>::KEYS);
+}
+int64_t decode_blocks(const DeviceInfo& dev, int rows) { return int64_t(dev.num_sms) * (rows == 8 ? 2 : 1); }
 
-template <int FMT, int D, bool Q8>
-cudaError_t launch_decode_typed(const DecodeParams& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
-  using Cfg = DecodeCfg<D, Q8>;
+template <int FMT, int D, bool Q8, int NB>
+cudaError_t launch_decode_rows(const DecodeParams& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
+  using Cfg = DecodeCfg<D, Q8, NB>;
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
-  auto kern = attention_decode_kernel<FMT, D, Q8>;
-  static unsigned long long smem_set = 0;
+  auto kern = attention_decode_kernel<FMT, D, Q8, NB>;
+  static unsigned long long smem_set = 0, carve_set = 0;
   cudaError_t e = set_smem_once(kern, int(Cfg::SMEM), smem_set);
+  // all of the SM's shared memory, or fewer than PER_SM blocks would share it
+  if (e == cudaSuccess)
+    e = set_attribute_once(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared, carve_set);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a.blocks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(Cfg::THREADS);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -822,29 +940,43 @@ cudaError_t launch_decode_typed(const DecodeParams& a, const CUtensorMap& tk, co
   return cudaLaunchKernelEx(&cfg, attention_decode_combine<T, D>, a);
 }
 
+template <int FMT, int D, bool Q8>
+cudaError_t launch_decode_typed(const DecodeParams& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
+  return a.rows == 8 ? launch_decode_rows<FMT, D, Q8, 1>(a, tk, tv, s) : launch_decode_rows<FMT, D, Q8, 2>(a, tk, tv, s);
+}
+
 }  // namespace
+
+// More tiles than any lengths can make of the problem (64 keys, 8 rows each).
+double most_tiles(const SeqProblem& p) {
+  const double rows = double(p.tokens_q) * p.group / 8 + p.batch;
+  const double keys = double(p.table != nullptr ? p.max_keys : p.tokens_kv) / 64 + 1;
+  return rows * keys * p.heads_kv;
+}
 
 bool seq_decode_ok(const SeqProblem& p, int dtype, int kv_dtype) {
   return (dtype == CMPX_F16 || dtype == CMPX_BF16) && (p.d == 64 || p.d == 128) && seq_tma_ok(p, kv_dtype) &&
          seq_rows_ok(p.Q, p.q_token, p.tokens_q, 8) && seq_rows_ok(p.Q, p.q_head, p.heads_q, 8) &&
-         (int64_t(p.tokens_q) * p.heads_q + 3) / 4 <= 0x7fffffffLL;
+         (int64_t(p.tokens_q) * p.heads_q + 3) / 4 <= 0x7fffffffLL && most_tiles(p) < 0x7fffffff;
 }
 
-size_t seq_decode_workspace(const SeqProblem& p, const DeviceInfo& dev) {
-  return size_t(decode_blocks(dev)) * 2 * 16 * (size_t(p.d) * 4 + 8) + (size_t(p.batch) + 2) * 8;
+size_t seq_decode_workspace(const SeqProblem& p, int rows, const DeviceInfo& dev) {
+  return size_t(decode_blocks(dev, rows)) * 2 * size_t(rows) * (size_t(p.d) * 4 + 8) + (size_t(p.batch) + 2) * 4;
 }
 
-cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, void* ws, const DeviceInfo& dev, int* err,
-                              cudaStream_t s) {
+cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, int rows, void* ws, const DeviceInfo& dev,
+                              int* err, cudaStream_t s) {
   const bool paged = p.table != nullptr, q8 = kv_dtype == CMPX_E4M3;
   DecodeParams a = {};
   a.p = p;
-  a.box_rows = paged && p.page_size < kKeys ? p.page_size : kKeys;
-  a.blocks = int(decode_blocks(dev));
+  a.rows = rows;
+  a.keys = decode_keys(p, q8);
+  a.box_rows = paged && p.page_size < a.keys ? p.page_size : a.keys;
+  a.blocks = int(decode_blocks(dev, rows));
   a.min_tiles = 1;
   a.part_o = static_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(a.blocks) * 2 * 16 * p.d);
-  a.plan = reinterpret_cast<int64_t*>(a.part_ml + int64_t(a.blocks) * 2 * 16);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(a.blocks) * 2 * rows * p.d);
+  a.plan = reinterpret_cast<int*>(a.part_ml + int64_t(a.blocks) * 2 * rows);
   a.err = err;
   CUtensorMap tk, tv;
   if (!seq_kv_maps(p, kv_dtype, a.box_rows, true, &tk, &tv)) return cudaErrorInvalidValue;

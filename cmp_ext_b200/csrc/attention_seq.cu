@@ -202,6 +202,7 @@ SeqProblem resolve_seq(const cmpx_attention_seq_args* a) {
     p.page_size = int(a->page_size);
     p.pages = int(a->pages);
     p.max_keys = int(a->max_pages * a->page_size);
+    while ((2 << p.page_lg) <= p.page_size) ++p.page_lg;
   }
   p.scale_log2 = a->scale * kLog2e;
   p.causal = a->causal != 0;
@@ -209,9 +210,19 @@ SeqProblem resolve_seq(const cmpx_attention_seq_args* a) {
   return p;
 }
 
+// Query rows a kv head has in a typical sequence: those of the longest one if
+// the caller or the layout says so, else of the mean one.
+int64_t typical_rows(const cmpx_attention_seq_args* a, const SeqProblem& p) {
+  const int64_t tokens = a->cu_seqlens_q == nullptr ? p.uniform_n
+                         : a->max_seqlen_q > 0      ? a->max_seqlen_q
+                         : a->batch > 0             ? (a->tokens_q + a->batch - 1) / a->batch
+                                                    : 0;
+  return tokens > INT_MAX ? INT_MAX : tokens * p.group;
+}
+
 // The kernel that runs a checked, non-empty problem, or -1.  Few query rows a
-// kv head run the flash-decoding kernel, whose blocks take 16 of them; more
-// the tcgen05 kernel.  Without a hint the mean length decides.
+// kv head run the flash-decoding kernel, whose units hold at most 16 of them;
+// more the tcgen05 kernel.
 int seq_path(const cmpx_attention_seq_args* a, const SeqProblem& p) {
   const bool simt_ok = a->head_dim <= kSimtMaxD && (a->tokens_q * a->heads_q + 3) / 4 <= INT_MAX;
   const bool tile_ok = seq_tile_ok(p, a->dtype, a->kv_dtype);
@@ -219,16 +230,16 @@ int seq_path(const cmpx_attention_seq_args* a, const SeqProblem& p) {
   if (a->path == CMPX_PATH_SIMT) return simt_ok ? CMPX_PATH_SIMT : -1;
   if (a->path == CMPX_PATH_TC) return tile_ok ? CMPX_PATH_TC : -1;
   if (a->path == CMPX_PATH_SKINNY) return decode_ok ? CMPX_PATH_SKINNY : -1;
-  const int64_t longest = a->cu_seqlens_q == nullptr ? p.uniform_n
-                          : a->max_seqlen_q > 0      ? a->max_seqlen_q
-                          : a->batch > 0             ? (a->tokens_q + a->batch - 1) / a->batch
-                                                     : 0;
-  if (decode_ok && (longest * p.group <= 16 || !tile_ok)) return CMPX_PATH_SKINNY;
+  if (decode_ok && (typical_rows(a, p) <= 16 || !tile_ok)) return CMPX_PATH_SKINNY;
   return tile_ok ? CMPX_PATH_TC : simt_ok ? CMPX_PATH_SIMT : -1;
 }
 
-size_t seq_workspace(const SeqProblem& p, int path, const DeviceInfo& dev) {
-  return path == CMPX_PATH_TC ? seq_tile_workspace(p, dev) : path == CMPX_PATH_SKINNY ? seq_decode_workspace(p, dev) : 0;
+int decode_rows(const cmpx_attention_seq_args* a, const SeqProblem& p) { return typical_rows(a, p) <= 8 ? 8 : 16; }
+
+size_t seq_workspace(const cmpx_attention_seq_args* a, const SeqProblem& p, int path, const DeviceInfo& dev) {
+  return path == CMPX_PATH_TC       ? seq_tile_workspace(p, dev)
+         : path == CMPX_PATH_SKINNY ? seq_decode_workspace(p, decode_rows(a, p), dev)
+                                    : 0;
 }
 
 }  // namespace
@@ -242,8 +253,13 @@ bool seq_tma_ok(const SeqProblem& p, int kv_dtype) {
   const bool paged = p.table != nullptr;
   if (paged && (p.page_size < 8 || (p.page_size & (p.page_size - 1)) != 0)) return false;
   if (paged ? (p.pages == 0 || p.max_keys == 0) : p.tokens_kv == 0) return false;  // no key at all
-  const int64_t unit = kv_dtype == CMPX_E4M3 ? 16 : 8;
+  const bool q8 = kv_dtype == CMPX_E4M3;
+  const int64_t unit = q8 ? 16 : 8;
   for (const SeqKV* x : {&p.k, &p.v}) {
+    // a page's scales are copied in 16-byte units
+    if (q8 && (p.page_size < 16 || !seq_rows_ok(x->scale, x->s_head, p.heads_kv, 16) ||
+               !seq_rows_ok(x->scale, x->s_page, p.pages, 16) || x->s_row != 1))
+      return false;
     if (!seq_rows_ok(x->base, x->row, paged ? p.page_size : p.tokens_kv, unit) ||
         !seq_rows_ok(x->base, x->head, p.heads_kv, unit) || (paged && !seq_rows_ok(x->base, x->page, p.pages, unit)))
       return false;
@@ -295,13 +311,14 @@ extern "C" int cmpx_attention_seq(const cmpx_attention_seq_args* args, cmpx_stre
   int* err = nullptr;
   st = device_facts(&dev, &err);
   if (st != CMPX_OK) return st;
-  const size_t need = seq_workspace(p, path, dev);
+  const size_t need = seq_workspace(args, p, path, dev);
   if (need > 0 && (args->workspace == nullptr || reinterpret_cast<uintptr_t>(args->workspace) % 16 != 0))
     return CMPX_ERR_INVALID_ARG;
   if (args->workspace_bytes < need) return CMPX_ERR_WORKSPACE;
   const cudaError_t e =
       path == CMPX_PATH_SKINNY
-          ? launch_seq_decode(p, args->dtype, args->kv_dtype, args->workspace, dev, err, stream)
+          ? launch_seq_decode(p, args->dtype, args->kv_dtype, decode_rows(args, p), args->workspace, dev, err,
+                              stream)
       : path == CMPX_PATH_TC ? launch_seq_tile(p, args->dtype, args->kv_dtype, args->workspace, dev, err, stream)
                            : launch_seq_simt(p, args->dtype, args->kv_dtype, stream);
   return e == cudaSuccess ? CMPX_OK : CMPX_ERR_CUDA;
@@ -314,7 +331,7 @@ extern "C" size_t cmpx_attention_seq_workspace_size(const cmpx_attention_seq_arg
   DeviceInfo dev;
   int* err = nullptr;
   if (device_facts(&dev, &err) != CMPX_OK) return 0;
-  return seq_workspace(p, seq_path(args, p), dev);
+  return seq_workspace(args, p, seq_path(args, p), dev);
 }
 
 extern "C" int cmpx_attention_seq_select_path(const cmpx_attention_seq_args* args) {

@@ -27,6 +27,7 @@ struct SeqProblem {
   int64_t table_stride;
   int batch, uniform_n, tokens_q, tokens_kv, heads_q, heads_kv, group, d;
   int page_size, pages, max_keys;  // max_keys: keys a row of the page table can name
+  int page_lg;                     // log2 page_size where that is whole (the TMA kernels')
   float scale_log2;                // scale * log2 e
   int causal, zero_rest;
 };
@@ -96,9 +97,10 @@ bool seq_kv_maps(const SeqProblem& p, int kv_dtype, int box_rows, bool swizzled,
 
 // flash-decoding kernel (attention_decode.cu)
 bool seq_decode_ok(const SeqProblem& p, int dtype, int kv_dtype);
-size_t seq_decode_workspace(const SeqProblem& p, const DeviceInfo& dev);
-cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, void* ws, const DeviceInfo& dev, int* err,
-                              cudaStream_t s);
+size_t seq_decode_workspace(const SeqProblem& p, int rows, const DeviceInfo& dev);
+// rows: 8 or 16 query rows share a pass over the keys
+cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, int rows, void* ws, const DeviceInfo& dev,
+                              int* err, cudaStream_t s);
 
 // tcgen05 kernel (attention_tile.cu)
 bool seq_tile_ok(const SeqProblem& p, int dtype, int kv_dtype);

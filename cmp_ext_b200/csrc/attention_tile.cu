@@ -65,7 +65,7 @@ struct TileCfg {
   static constexpr int VS = D == 64 ? 4 : 2;
   static constexpr int RS = !Q8 ? 0 : D == 64 ? 4 : 2;
   static constexpr int RAW = 128 * D;
-  static constexpr size_t SMEM = size_t(TILE) * (2 + KS + VS) + size_t(RS) * RAW + 1024 + 512;
+  static constexpr size_t SMEM = size_t(TILE) * (2 + KS + VS) + size_t(RS) * (RAW + 128) + 1024 + 512;
   // registers a thread of the two softmax warpgroups and of the others
   // (setmaxnreg), out of the block's 3 x 168 or 4 x 128 at launch
   static constexpr int REGS_SOFTMAX = Q8 ? 184 : 216, REGS_OTHER = 72;
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
   uint8_t* sK = sQ + 2 * Cfg::TILE;         // [KS]
   uint8_t* sV = sK + KS * Cfg::TILE;        // [VS]
   uint8_t* sR = sV + VS * Cfg::TILE;        // [RS] raw codes
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sR + Cfg::RS * Cfg::RAW);
+  uint8_t* sScale = sR + Cfg::RS * Cfg::RAW;  // [RS][128] their e8m0 bytes
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sScale + Cfg::RS * 128);
   uint64_t* q_full = bars;
   uint64_t* k_full = q_full + 1;    // [KS]
   uint64_t* k_empty = k_full + KS;  // [KS]
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
       auto page_of = [&](int j) -> int {
         const int key = (jb + j) * 128 + lane * a.box_rows;
         if (table == nullptr || lane >= boxes_full || key >= kend) return 0;
-        return __ldg(table + key / p.page_size);
+        return __ldg(table + (key >> p.page_lg));
       };
       int page = page_of(0), kdone = 0, vdone = 0;
       bool ok = true;
@@ -354,13 +355,26 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
             ok = false;
             break;
           }
-          if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(boxes * a.box_rows * D * (Q8 ? 1 : 2)));
+          // scales of pages that are none: zeros, as TMA gives for their codes
+          const bool there = lane < boxes && page >= 0 && page < p.pages;
+          uint32_t bytes = uint32_t(boxes * a.box_rows * D * (Q8 ? 1 : 2));
+          uint8_t* sdst = sScale + ((2 * j + v) % RS) * 128 + lane * a.box_rows;
+          if constexpr (Q8) {
+            if (lane < boxes && !there)
+              for (int k = 0; k < a.box_rows; k += 4) *reinterpret_cast<uint32_t*>(sdst + k) = 0u;
+            bytes += uint32_t(__popc(__ballot_sync(0xffffffffu, there)) * a.box_rows);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(full, bytes);
           __syncwarp();
           if (lane < boxes) {
             const CUtensorMap* m = v ? &tmV : &tmK;
-            const int row = table != nullptr ? (kv0 + lane * a.box_rows) % p.page_size : s.k0 + kv0;
+            const int row = table != nullptr ? (kv0 + lane * a.box_rows) & (p.page_size - 1) : s.k0 + kv0;
             if constexpr (Q8) {
+              const SeqKV& kv = v ? p.v : p.k;
               tma_load_4d(dst + lane * a.box_rows * D, m, full, 0, row, hk, page);
+              if (there)
+                bulk_load(sdst, kv.scale + page * kv.s_page + hk * kv.s_head + row, uint32_t(a.box_rows), full);
             } else {
 #pragma unroll
               for (int c = 0; c < Cfg::QCH; ++c)
@@ -488,23 +502,10 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
       constexpr int LPR = D / 16, RPI = 128 / LPR;  // lanes a row, rows a pass of the 128 threads
       const int tid = int(threadIdx.x) - 384;
       const int c16 = tid % LPR, r_in = tid / LPR;
-      const int* table = p.table + seq * p.table_stride;
       bool ok = true;
       for (int i = 0; i < 2 * nkv && ok; ++i) {
         const int j = i >> 1, kv0 = (jb + j) * 128;
         const bool isv = (i & 1) != 0;
-        const SeqKV& kv = isv ? p.v : p.k;
-        float up[128 / RPI];
-#pragma unroll
-        for (int k = 0; k < 128 / RPI; ++k) {
-          const int key = kv0 + k * RPI + r_in;
-          up[k] = 0.0f;  // rows behind the last key, and pages that are none: zeros
-          if (key < kend) {
-            const int page = __ldg(table + key / p.page_size);
-            if (page >= 0 && page < p.pages)
-              up[k] = e8m0_to_float(__ldg(kv.scale + page * kv.s_page + hk * kv.s_head + (key % p.page_size) * kv.s_row));
-          }
-        }
         const int r = i % RS, slot = isv ? j % VS : j % KS, use = isv ? j / VS : j / KS;
         ok = __all_sync(0xffffffffu, mbar_wait(&r_full[r], (i / RS) & 1, abort_flag) &&
                                          mbar_wait(isv ? &v_empty[slot] : &k_empty[slot], (use & 1) ^ 1, abort_flag));
@@ -518,14 +519,16 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
         for (int k = 0; k < 128 / RPI; ++k) {
           const int row = k * RPI + r_in;
           const uint4 codes = *reinterpret_cast<const uint4*>(src + row * D + c16 * 16);
+          // a row behind the last key may hold anything, NaN too: zeros
+          const bool in = kv0 + row < kend;
+          const float up = in ? e8m0_to_float(sScale[r * 128 + row]) : 0.0f;
           const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
           uint32_t h[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            // a row that counts as zeros may hold anything, NaN codes too
-            const uint32_t x = kv0 + row < kend ? w[e] : 0u;
-            h[2 * e] = dequant2(x & 0xffffu, up[k], (T*)nullptr);
-            h[2 * e + 1] = dequant2(x >> 16, up[k], (T*)nullptr);
+            const uint32_t x = in ? w[e] : 0u;
+            h[2 * e] = dequant2(x & 0xffffu, up, (T*)nullptr);
+            h[2 * e + 1] = dequant2(x >> 16, up, (T*)nullptr);
           }
           const int unit = (c16 & 3) * 2, flip = c16 >> 2;
           uint8_t* at = dst + (c16 >> 2) * 16384 + row * 128;

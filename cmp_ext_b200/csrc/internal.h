@@ -174,19 +174,24 @@ inline void apply_pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int us
 }  // namespace cmpx
 
 namespace cmpx {
-// Sets a kernel's dynamic shared-memory limit once per device (the attribute
-// is per function and device; setting it on every launch costs host time that
-// shows up in short kernels' latency).  `done` must be a flag word owned by
-// that one kernel (a static in its launcher): bit d = set on device d.
+// Sets a kernel's attribute once per device (attributes are per function and
+// device; setting one on every launch costs host time that shows up in short
+// kernels' latency).  `done` must be a flag word owned by that one kernel and
+// attribute (a static in its launcher): bit d = set on device d.
 template <typename KernelPtr>
-cudaError_t set_smem_once(KernelPtr kern, int bytes, unsigned long long& done) {
+cudaError_t set_attribute_once(KernelPtr kern, cudaFuncAttribute attr, int value, unsigned long long& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const unsigned long long bit = dev < 64 ? (1ull << dev) : 0ull;
   if (bit != 0 && (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  e = cudaFuncSetAttribute(kern, attr, value);
   if (e == cudaSuccess && bit != 0) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
   return e;
+}
+// The dynamic shared-memory limit.
+template <typename KernelPtr>
+cudaError_t set_smem_once(KernelPtr kern, int bytes, unsigned long long& done) {
+  return set_attribute_once(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes, done);
 }
 }  // namespace cmpx
