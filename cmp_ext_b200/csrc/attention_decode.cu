@@ -17,14 +17,16 @@
 // sixteen would, and a warp's state (D x 8 sums) leaves registers for sixteen
 // warps an SM, which is what hides the latency of the strip's chain of
 // dependent steps (with rows along the 16-wide side, twice the products and
-// eight warps, an e4m3 tile took 5200 cycles, now NNNN).
+// eight warps, an e4m3 tile took 5200 cycles; now 1400).
 //
 // Work: units (sequence, kv head, ROWS rows) of ceil(keys / 64) tiles in one
-// list of W tiles; block c of P takes tiles [c W / P, (c + 1) W / P), so
-// ragged lengths and few sequences load every SM alike, and its loads run
-// ahead across unit borders.  A unit that lies in one block is finished
-// there; the pieces of the others (at most two a block) go to the workspace
-// and attention_decode_combine joins them in order of their keys.
+// list, each unit's beginning and end weighted like two tiles; block c of P
+// takes the places [c W / P, (c + 1) W / P) of W, so ragged lengths and few
+// sequences load every SM alike, and its loads run ahead across unit borders.
+// A unit that lies in one block is finished there; the pieces of the others
+// (at most two a block) go to the workspace and attention_decode_combine joins
+// them in order of their keys.  Where no sequence can be long, blocks take
+// whole units and the second kernel is spared.
 //
 // The last warp loads (TMA; lane i box i, a page or the whole tile, and with
 // an 8-bit cache its scales; a chunk of pages looked up ahead); the others
@@ -62,7 +64,7 @@ struct DecodeParams {
   SeqProblem p;
   int box_rows;     // keys of one TMA box
   int blocks;       // most blocks that share the work
-  int min_tiles;    // tiles worth a block
+  int whole;        // no unit is split: a block takes whole ones, and no second kernel runs
   int rows;         // of a unit: 8 or 16
   int keys;         // of a tile
   float* part_o;    // [blocks][2][rows][D]
@@ -119,13 +121,21 @@ __device__ __forceinline__ int unit_tiles(const DecodeParams& a, int len) { retu
 __device__ __forceinline__ int row_tiles(const DecodeParams& a, int n) {
   return (n * a.p.group + a.rows - 1) / a.rows;
 }
-// First tile of block c: floor(c * total / used), c <= used <= 4096.
-__device__ __forceinline__ int first_tile(int c, int total, int used) {
+// What a unit counts for in the list that the blocks share: its tiles and
+// kUnitCost for its beginning and end (queries to load, warps to join: about
+// as long as two tiles take a block), or one where no unit is split.
+constexpr int kUnitCost = 2;
+__device__ __forceinline__ int unit_weight(const DecodeParams& a, int nt) { return a.whole ? 1 : nt + kUnitCost; }
+// Tile that place x of a unit's weight stands for: the first kUnitCost + 1
+// places are the first tile's.
+__device__ __forceinline__ int place_tile(const DecodeParams& a, int x) { return a.whole ? 0 : max(x - kUnitCost, 0); }
+// First place of block c: floor(c * total / used).
+__device__ __forceinline__ int first_place(int c, int total, int used) {
   const int q = total / used;
-  return c * q + c * (total - q * used) / used;
+  return c * q + int(int64_t(c) * (total - q * used) / used);
 }
 
-// A place in the list of tiles.
+// A tile in the list.
 struct Walk {
   int b, hk, rt, j;  // sequence, kv head, row tile, tile of the unit
   int nrt, nt;       // row tiles, tiles of a unit
@@ -135,8 +145,17 @@ struct Walk {
     nrt = row_tiles(a, s.n);
     nt = unit_tiles(a, s.len);
   }
-  __device__ __forceinline__ void step(const DecodeParams& a) {
-    if (++j < nt) return;
+  // The tile at place `rel` of sequence `seq`.
+  __device__ __forceinline__ void at(const DecodeParams& a, int seq, int rel) {
+    b = seq;
+    enter(a);
+    const int weight = unit_weight(a, nt), per_head = nrt * weight;
+    hk = rel / per_head;
+    rel -= hk * per_head;
+    rt = rel / weight;
+    j = place_tile(a, rel - rt * weight);
+  }
+  __device__ __forceinline__ void next_unit(const DecodeParams& a) {
     j = 0;
     if (++rt < nrt) return;
     rt = 0;
@@ -147,6 +166,7 @@ struct Walk {
       enter(a);
     } while (nrt == 0);
   }
+  __device__ __forceinline__ bool is(const Walk& x) const { return b == x.b && hk == x.hk && rt == x.rt && j == x.j; }
 };
 
 // What the loading warp tells the others of a tile; one lies beside each of
@@ -162,11 +182,10 @@ struct alignas(16) TileInfo {
   int q0, n, k0;     // of Seq
   int pad[2];
 };
-constexpr int kBegins = 1;   // the piece's first tile
-constexpr int kEnds = 2;     // its last one
-constexpr int kWhole = 4;    // the piece is the whole unit
-constexpr int kFirst = 8;    // the unit begins in this block
-constexpr int kLast = 16;    // the block's last tile
+constexpr int kEnds = 1;     // the piece's last tile
+constexpr int kWhole = 2;    // the piece is the whole unit
+constexpr int kFirst = 4;    // the unit begins in this block
+constexpr int kLast = 8;     // the block's last tile
 
 // Query row r of a unit: its token, head, and visible keys (0: no such row).
 struct Row {
@@ -199,13 +218,13 @@ struct DecodeCfg {
   static constexpr int RING = 196608 / PER_SM / (2 * HALF);
   static constexpr int STAGES = RING < 8 ? RING : 8;
   static constexpr int SCALES = Q8 ? 2 * KEYS : 0;     // a tile's e8m0 bytes
-  static constexpr int SLOTS = NB == 1 ? 3 : 2;        // sums of a piece that meet in shared memory
-  static constexpr int MERGE = SLOTS * ROWS * D * 4;
-  static constexpr size_t SMEM = size_t(STAGES) * (2 * HALF + SCALES) + MERGE + STAGES * sizeof(TileInfo) + 1024 + 256 + WARPS * ROWS * 8;
+  static constexpr int SLOTS = NB == 1 ? WARPS : 4;    // warps whose rows of a piece fit a place of the ring
+  static_assert(SLOTS * ROWS * D * 4 <= 2 * HALF, "a piece's rows fit a place of the ring");
+  static constexpr size_t SMEM = size_t(STAGES) * (2 * HALF + SCALES) + STAGES * sizeof(TileInfo) + 1024 + 256 + 2 * WARPS * ROWS * 8;
   static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory budget");
 };
 
-// Place of row r, column d among joined rows: the eight rows a store
+// Place of row r, column d of a warp's rows: the eight rows a store
 // instruction touches lie on different banks.
 template <int D>
 __device__ __forceinline__ int merge_at(int r, int d) {
@@ -215,7 +234,7 @@ __device__ __forceinline__ int merge_at(int r, int d) {
 // One row over keys [kbeg, kend) from its definition; a warp computes it.
 template <typename T, int D, bool Q8>
 __device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk, const T* q, int kbeg, int kend,
-                                      float m, float* merge, int r) {
+                                      float m, float (&acc)[D / 32]) {
   const int lane = threadIdx.x & 31;
   constexpr int NV = D / 32;
   using KV = typename std::conditional<Q8, __nv_fp8_e4m3, T>::type;
@@ -223,7 +242,6 @@ __device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int
     if constexpr (Q8) return float(*at);
     else return ldf(at);
   };
-  float acc[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
   for (int j = kbeg; j < kend; ++j) {
@@ -250,8 +268,6 @@ __device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int
 #pragma unroll
     for (int i = 0; i < NV; ++i) acc[i] = fmaf(w, load(vr + lane + 32 * i), acc[i]);
   }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) merge[merge_at<D>(r, lane + 32 * i)] = acc[i];
 }
 
 template <int FMT, int D, bool Q8, int NB>
@@ -269,16 +285,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024 - (raw & 1023)) & 1023);
   uint8_t* ring = smem;                                                        // [STAGES] keys, values
-  float* merge = reinterpret_cast<float*>(ring + size_t(STAGES) * 2 * HALF);   // [SLOTS][ROWS][D]
-  uint8_t* scales = reinterpret_cast<uint8_t*>(merge) + Cfg::MERGE;            // [STAGES][2][KEYS]
+  uint8_t* scales = ring + size_t(STAGES) * 2 * HALF;                          // [STAGES][2][KEYS]
   TileInfo* infos = reinterpret_cast<TileInfo*>(scales + STAGES * Cfg::SCALES);  // [STAGES]
   uint64_t* full = reinterpret_cast<uint64_t*>(infos + STAGES);
   uint64_t* empty = full + STAGES;
   uint64_t* join = empty + STAGES;  // the consumers meet
   volatile int* abort_flag = reinterpret_cast<volatile int*>(join + 1);
-  int* start = const_cast<int*>(abort_flag) + 1;                               // [2] sequence, place in it
-  int* warp_sum = start + 2;                                                   // [WARPS + 1]
-  float2* ml = reinterpret_cast<float2*>(warp_sum + 13);                       // [WARPS][ROWS]
+  int* start = const_cast<int*>(abort_flag) + 1;                               // [2][2] sequence, place in it
+  int* warp_sum = start + 4;                                                   // [WARPS + 1]
+  float2* ml = reinterpret_cast<float2*>(warp_sum + 13);                       // [2][WARPS][ROWS]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -294,8 +309,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
   pdl_trigger();
   pdl_wait();
 
-  // ---- this block's share of the tiles.  Sequences are counted THREADS at a
-  // time; `mine` (tiles of this thread's sequence) and `upto` (of all up to
+  // ---- this block's share of the list.  Sequences are counted THREADS at a
+  // time; `mine` (the weight of this thread's sequence) and `upto` (of all up to
   // it) stay in registers where one pass holds them all.
   int mine = 0, upto = 0;
   auto count_pass = [&](int base) -> int {
@@ -303,7 +318,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
     mine = 0;
     if (b < p.batch) {
       const Seq s = seq_of(p, b);
-      mine = row_tiles(a, s.n) * unit_tiles(a, s.len) * p.heads_kv;
+      mine = row_tiles(a, s.n) * unit_weight(a, unit_tiles(a, s.len)) * p.heads_kv;
     }
     upto = mine;
 #pragma unroll
@@ -325,39 +340,40 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
   int total = 0;
   for (int base = 0; base < p.batch; base += THREADS) {
     const int all = count_pass(base);
-    if (blockIdx.x == 0 && base + int(threadIdx.x) < p.batch) a.plan[base + threadIdx.x] = total + upto - mine;
+    if (blockIdx.x == 0 && !a.whole && base + int(threadIdx.x) < p.batch) a.plan[base + threadIdx.x] = total + upto - mine;
     total += all;
   }
-  const int used = min((total + a.min_tiles - 1) / a.min_tiles, a.blocks);
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  const int used = min(total, a.blocks);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && !a.whole) {
     a.plan[p.batch] = total;
     a.plan[p.batch + 1] = used;
   }
+  // the places of its first tile and of the next block's
   const int c_id = int(blockIdx.x);
-  const int lo = c_id < used ? first_tile(c_id, total, used) : 0;
-  const int count = c_id < used ? first_tile(c_id + 1, total, used) - lo : 0;  // tiles of this block
-  for (int base = 0, before = 0; count > 0 && base < p.batch; base += THREADS) {
+  const int lo = c_id < used ? first_place(c_id, total, used) : 0;
+  const int hi = c_id < used ? first_place(c_id + 1, total, used) : 0;
+  for (int base = 0, before = 0; lo < hi && base < p.batch; base += THREADS) {
     int all = total;
     if (p.batch > THREADS) all = count_pass(base);
-    const int rel = lo - (before + upto - mine);
-    if (rel >= 0 && rel < mine) {
-      start[0] = base + int(threadIdx.x);
-      start[1] = rel;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int rel = (e ? hi : lo) - (before + upto - mine);
+      if (rel >= 0 && rel < mine) {
+        start[2 * e] = base + int(threadIdx.x);
+        start[2 * e + 1] = rel;
+      }
     }
     before += all;
-    if (lo < before) break;
+    if (hi < before) break;
   }
   __syncthreads();
-  Walk w = {};
-  if (count > 0) {
-    w.b = start[0];
-    int rel = start[1];
-    w.enter(a);
-    const int per_head = w.nrt * w.nt;
-    w.hk = rel / per_head;
-    rel -= w.hk * per_head;
-    w.rt = rel / w.nt;
-    w.j = rel - w.rt * w.nt;
+  bool busy = lo < hi;
+  Walk w = {}, end = {};
+  if (busy) {
+    w.at(a, start[0], start[1]);
+    end.b = p.batch;
+    if (hi < total) end.at(a, start[2], start[3]);
+    busy = !w.is(end);
   }
 
   if (warp == WARPS) {
@@ -375,23 +391,33 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       return p.table != nullptr && (int64_t(at) << p.page_lg) < x.s.len ? __ldg(p.table + x.b * p.table_stride + at) : 0;
     };
     int chunk = -1, page32 = 0, next32 = 0;
-    if (count > 0) next32 = pages_of(w, (w.j * KEYS) >> p.page_lg >> 5);
-    int st = 0;
+    if (busy) next32 = pages_of(w, (w.j * KEYS) >> p.page_lg >> 5);
+    int st = 0, piece_key = w.j * KEYS;
     uint32_t phase = 1;
     int done = 0;
-    bool ok = true;
-    for (int i = 0; i < count; ++i) {
+    bool ok = true, begins = true, last = !busy;
+    while (!last) {
       const int first = (w.j * KEYS) >> p.page_lg;  // page of the tile's first key
-      if (w.j == 0 || first >> 5 != chunk) {
+      if (begins || first >> 5 != chunk) {
         chunk = first >> 5;
         page32 = next32;
         if ((int64_t(chunk + 1) << p.page_lg << 5) < w.s.len) {
           next32 = pages_of(w, chunk + 1);
-        } else if (i + w.nt - w.j < count) {
+        } else {
           Walk x = w;
-          x.j = x.nt - 1;
-          x.step(a);
-          next32 = pages_of(x, 0);
+          x.next_unit(a);
+          if (x.b < p.batch) next32 = pages_of(x, 0);
+        }
+        if (begins) {
+          // the queries' way from memory begins before the tile's own: a
+          // 128-byte line a lane, rows of a unit in turn
+          constexpr int LINES = D * 2 / 128;
+          const int q = w.rt * a.rows + lane / LINES, token = q / p.group;
+          if (lane < a.rows * LINES && token < w.s.n) {
+            const T* at = static_cast<const T*>(p.Q) + int64_t(w.s.q0 + token) * p.q_token +
+                          int64_t(w.hk * p.group + q - token * p.group) * p.q_head + lane % LINES * 64;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+          }
         }
       }
       const int now = __shfl_sync(0xffffffffu, page32, first + lane);  // (modulo 32)
@@ -399,9 +425,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       TileInfo info;
       info.key = kv0;
       info.len = w.s.len;
-      info.flags = (i == 0 || w.j == 0 ? kBegins : 0) | (i + 1 == count || w.j + 1 == w.nt ? kEnds : 0) |
-                   (i >= w.j ? kFirst : 0) | (i >= w.j && w.j + 1 == w.nt ? kWhole : 0) | (i + 1 == count ? kLast : 0);
-      info.piece_key = i >= w.j ? 0 : (w.j - i) * KEYS;
+      info.piece_key = piece_key;
       info.b = w.b;
       info.hk = hk;
       info.row0 = w.rt * a.rows;
@@ -409,7 +433,14 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       info.n = w.s.n;
       info.k0 = k0;
       const int boxes = min(boxes_full, (w.s.len - kv0 + a.box_rows - 1) / a.box_rows);
-      if (i + 1 < count) w.step(a);
+      const bool unit_ends = w.j + 1 == w.nt;
+      if (unit_ends) w.next_unit(a);
+      else ++w.j;
+      last = w.is(end) || w.b >= p.batch;
+      info.flags = (unit_ends || last ? kEnds : 0) | (piece_key == 0 ? kFirst : 0) |
+                   (piece_key == 0 && unit_ends ? kWhole : 0) | (last ? kLast : 0);
+      begins = unit_ends;
+      if (unit_ends) piece_key = 0;
       if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], phase, abort_flag))) {
         if (lane == 0) rec_err(a.err, abort_flag, kDevTimeoutEmpty);
         ok = false;
@@ -484,15 +515,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       else return base ^ (2 * i << 4);
     };
     constexpr int PITCH = Cfg::ROW < 128 ? 64 : 128;
-    uint32_t qf[DT][NB][2];               // Q^T: row g of block nb
-    float o[DT][NB][4];                   // O^T: two columns, rows 2t and 2t + 1
-    float m[NB][2], l[NB][2], qs[NB][2];  // rows 2t, 2t + 1: reference point, sum (this lane's keys), score factor
-    int lim[NB][2];
-    int lim_min = 0;                      // of all rows
-    float v_ref = 0.0f;                   // 8-bit: 1 / the scale that value scales are relative to (0: none yet)
     int strip = warp;                     // the next of this warp's strips, counted from the tile's first
-    int st = 0, flags = count > 0 ? 0 : kLast;
+    int st = 0, flags = busy ? 0 : kLast;
     uint32_t phase = 0, join_phase = 0;
+    int piece = 0;
     bool ok = true;
     auto meet = [&]() {
       __syncwarp();
@@ -500,15 +526,29 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       ok = __all_sync(0xffffffffu, mbar_wait(join, join_phase, abort_flag)) && ok;
       join_phase ^= 1u;
     };
-    while (ok && !(flags & kLast)) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, abort_flag))) {
-        ok = false;
-        break;
+    auto next_tile = [&]() {
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase, abort_flag));
+      if (ok) flags = infos[st].flags;
+    };
+    auto release = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      if (++st == STAGES) {
+        st = 0;
+        phase ^= 1u;
       }
-      const TileInfo& info = infos[st];
-      flags = info.flags;
-      if (flags & kBegins) {
-        v_ref = 0.0f;
+    };
+    while (!(flags & kLast)) {  // a piece of a unit
+      next_tile();
+      if (!ok) break;
+      uint32_t qf[DT][NB][2];               // Q^T: row g of block nb
+      float o[DT][NB][4];                   // O^T: two columns, rows 2t and 2t + 1
+      float m[NB][2], l[NB][2], qs[NB][2];  // rows 2t, 2t + 1: reference point, sum (this lane's keys), score factor
+      int lim[NB][2];
+      int lim_min;                          // of all rows
+      float v_ref = 0.0f;                   // 8-bit: 1 / the scale that value scales are relative to (0: none yet)
+      {
+        const TileInfo& info = infos[st];
         lim_min = info.len;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -569,275 +609,297 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[k][nb][e] = 0.0f;
       }
+      while (true) {  // a tile
 #pragma unroll 1
-      for (; strip < KEYS / 16; strip += WARPS) {
-        const int kv0 = info.key + strip * 16;
-        const int tail = info.len - kv0;  // keys of the strip
-        if (tail <= 0) continue;
-        const uint32_t kbase = smem_u32(ring) + st * 2 * HALF + strip * 16 * PITCH + lane_at, vbase = kbase + HALF;
-        // ---- scores: keys g and g + 8, rows 2t and 2t + 1; even and odd
-        // steps in chains of their own
-        float s2[2][NB][4];
+        for (; strip < KEYS / 16; strip += WARPS) {
+          const int kv0 = infos[st].key + strip * 16;
+          const int tail = infos[st].len - kv0;  // keys of the strip
+          if (tail <= 0) continue;
+          const uint32_t kbase = smem_u32(ring) + st * 2 * HALF + strip * 16 * PITCH + lane_at, vbase = kbase + HALF;
+          // ---- scores: keys g and g + 8, rows 2t and 2t + 1; even and odd
+          // steps in chains of their own
+          float s2[2][NB][4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s2[c][nb][e] = 0.0f;
-        if constexpr (!Q8) {
-#pragma unroll
-          for (int k = 0; k < DT; ++k) {
-            uint32_t b[4];
-            ldsm_x4(b, ldsm_at(kbase, k));
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) mma16<BF>(s2[k & 1][nb], b, qf[k][nb][0], qf[k][nb][1]);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < DT; k += 2) {
-            uint32_t b[4];  // keys 0-7 and 8-15 of units k and k + 1
-            ldsm_x4(b, ldsm_at(kbase, k / 2));
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint32_t f[4];
-              e4m3_to_half(b[2 * u], f[0], f[2]);
-              e4m3_to_half(b[2 * u + 1], f[1], f[3]);
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma16<false>(s2[u][nb], f, qf[k + u][nb][0], qf[k + u][nb][1]);
-            }
-          }
-        }
-        const uint8_t* sc = scales + st * Cfg::SCALES + strip * 16 + g;
-        float ks[2] = {1.0f, 1.0f};
-        if constexpr (Q8) {
-          ks[0] = e8m0_to_float(sc[0]);
-          ks[1] = e8m0_to_float(sc[8]);
-        }
-        // in log2 units; hidden scores -inf
-        float s[NB][4];
-        bool grew = false;
-        const bool cut = kv0 + 16 > lim_min;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[nb][e] = (s2[0][nb][e] + s2[1][nb][e]) * qs[nb][e & 1];
-            if constexpr (Q8) s[nb][e] *= ks[e >> 1];
-          }
-          if (cut) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]) s[nb][e] = -INFINITY;
-          }
-          grew = grew || fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kGrow || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kGrow;
-        }
-        if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float mx = fmaxf(s[nb][e], s[nb][e + 2]);
-#pragma unroll
-              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-              const bool up = mx > m[nb][e] + kGrow;
-              const float m_new = up ? mx - kBias : m[nb][e];
-              const float alpha = up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
-              m[nb][e] = m_new;
-              l[nb][e] *= alpha;
-#pragma unroll
-              for (int k = 0; k < DT; ++k) {
-                o[k][nb][e] *= alpha;
-                o[k][nb][e + 2] *= alpha;
-              }
-            }
-        }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[nb][e] = ex2_approx(s[nb][e] - m[nb][e & 1]);
-            l[nb][e & 1] += s[nb][e];
-          }
-        // ---- O^T += V^T P^T.  Value rows behind the last key may hold
-        // anything: their elements are cleared
-        auto keep = [&](int h) -> uint32_t {
-          return (8 * h + 2 * t < tail ? 0xffffu : 0u) | (8 * h + 2 * t + 1 < tail ? 0xffff0000u : 0u);
-        };
-        if constexpr (!Q8) {
-          auto add = [&](auto clear) {
-            uint32_t pf[NB][2];
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (T*)nullptr));
+              for (int e = 0; e < 4; ++e) s2[c][nb][e] = 0.0f;
+          if constexpr (!Q8) {
 #pragma unroll
             for (int k = 0; k < DT; ++k) {
               uint32_t b[4];
-              ldsm_x4_t(b, ldsm_at(vbase, k));
-              uint32_t f[4] = {b[0], b[2], b[1], b[3]};
-              if constexpr (decltype(clear)::value) {
+              ldsm_x4(b, ldsm_at(kbase, k));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] &= keep(e >> 1);
-              }
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma16<BF>(o[k][nb], f, pf[nb][0], pf[nb][1]);
+              for (int nb = 0; nb < NB; ++nb) mma16<BF>(s2[k & 1][nb], b, qf[k][nb][0], qf[k][nb][1]);
             }
-          };
-          if (tail < 16) add(std::true_type());
-          else add(std::false_type());
-        } else {
-          float vs[2];
-          vs[0] = e8m0_to_float(sc[KEYS]);
-          vs[1] = e8m0_to_float(sc[KEYS + 8]);
-          if (v_ref == 0.0f) {
-            float top = fmaxf(g < tail ? vs[0] : 0.0f, g + 8 < tail ? vs[1] : 0.0f);  // drops a NaN
+          } else {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            v_ref = 1.0f / fminf(fmaxf(top, 0x1p-126f), 0x1p126f);
+            for (int k = 0; k < DT; k += 2) {
+              uint32_t b[4];  // keys 0-7 and 8-15 of units k and k + 1
+              ldsm_x4(b, ldsm_at(kbase, k / 2));
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                uint32_t f[4];
+                e4m3_to_half(b[2 * u], f[0], f[2]);
+                e4m3_to_half(b[2 * u + 1], f[1], f[3]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) mma16<false>(s2[u][nb], f, qf[k + u][nb][0], qf[k + u][nb][1]);
+              }
+            }
           }
-          bool near = true;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            vs[h] = g + 8 * h < tail ? vs[h] * v_ref : 1.0f;
-            near = near && vs[h] >= 0x1p-10f && vs[h] <= 0x1p6f;
+          const uint8_t* sc = scales + st * Cfg::SCALES + strip * 16 + g;
+          float ks[2] = {1.0f, 1.0f};
+          if constexpr (Q8) {
+            ks[0] = e8m0_to_float(sc[0]);
+            ks[1] = e8m0_to_float(sc[8]);
           }
-          near = __all_sync(0xffffffffu, near);
+          // in log2 units; hidden scores -inf
+          float s[NB][4];
+          bool grew = false;
+          const bool cut = kv0 + 16 > lim_min;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+          for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)  // (a hidden key's scale may be a NaN, which is not near)
-              s[nb][e] = !near && s[nb][e] == 0.0f ? 0.0f : s[nb][e] * vs[e >> 1];
-          auto add = [&](auto half_type, auto clear) {
-            using P = decltype(half_type);
-            constexpr bool kBf = std::is_same<P, __nv_bfloat16>::value;
-            uint32_t pf[NB][2];
+            for (int e = 0; e < 4; ++e) {
+              s[nb][e] = (s2[0][nb][e] + s2[1][nb][e]) * qs[nb][e & 1];
+              if constexpr (Q8) s[nb][e] *= ks[e >> 1];
+            }
+            if (cut) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]) s[nb][e] = -INFINITY;
+            }
+            grew = grew || fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kGrow || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kGrow;
+          }
+          if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (P*)nullptr));
+              for (int e = 0; e < 2; ++e) {
+                float mx = fmaxf(s[nb][e], s[nb][e + 2]);
 #pragma unroll
-            for (int k = 0; k < DT; k += 2) {
-              uint32_t b[4];  // units k and k + 1, each keys 0-7 and 8-15
-              ldsm_x4_t(b, ldsm_at(vbase, k / 2));
+                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                const bool up = mx > m[nb][e] + kGrow;
+                const float m_new = up ? mx - kBias : m[nb][e];
+                const float alpha = up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
+                m[nb][e] = m_new;
+                l[nb][e] *= alpha;
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                // codes of two keys: even columns (rows 0-7 of the 16-wide
-                // side) together, and odd ones
-                uint32_t f[4];
-                e4m3_to_half(__byte_perm(b[2 * u], 0, 0x3120), f[0], f[1]);
-                e4m3_to_half(__byte_perm(b[2 * u + 1], 0, 0x3120), f[2], f[3]);
+                for (int k = 0; k < DT; ++k) {
+                  o[k][nb][e] *= alpha;
+                  o[k][nb][e + 2] *= alpha;
+                }
+              }
+          }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if constexpr (kBf) f[e] = half2_to_bf16(f[e]);
-                  if constexpr (decltype(clear)::value) f[e] &= keep(e >> 1);
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[nb][e] = ex2_approx(s[nb][e] - m[nb][e & 1]);
+              l[nb][e & 1] += s[nb][e];
+            }
+          // ---- O^T += V^T P^T.  Value rows behind the last key may hold
+          // anything: their elements are cleared
+          auto keep = [&](int h) -> uint32_t {
+            return (8 * h + 2 * t < tail ? 0xffffu : 0u) | (8 * h + 2 * t + 1 < tail ? 0xffff0000u : 0u);
+          };
+          if constexpr (!Q8) {
+            auto add = [&](auto clear) {
+              uint32_t pf[NB][2];
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (T*)nullptr));
+#pragma unroll
+              for (int k = 0; k < DT; ++k) {
+                uint32_t b[4];
+                ldsm_x4_t(b, ldsm_at(vbase, k));
+                uint32_t f[4] = {b[0], b[2], b[1], b[3]};
+                if constexpr (decltype(clear)::value) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) f[e] &= keep(e >> 1);
                 }
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mma16<kBf>(o[k + u][nb], f, pf[nb][0], pf[nb][1]);
+                for (int nb = 0; nb < NB; ++nb) mma16<BF>(o[k][nb], f, pf[nb][0], pf[nb][1]);
               }
+            };
+            if (tail < 16) add(std::true_type());
+            else add(std::false_type());
+          } else {
+            float vs[2];
+            vs[0] = e8m0_to_float(sc[KEYS]);
+            vs[1] = e8m0_to_float(sc[KEYS + 8]);
+            if (v_ref == 0.0f) {
+              float top = fmaxf(g < tail ? vs[0] : 0.0f, g + 8 < tail ? vs[1] : 0.0f);  // drops a NaN
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              v_ref = 1.0f / fminf(fmaxf(top, 0x1p-126f), 0x1p126f);
             }
-          };
-          if (!near) add(__nv_bfloat16(), std::true_type());
-          else if (tail < 16) add(__half(), std::true_type());
-          else add(__half(), std::false_type());
+            bool near = true;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              vs[h] = g + 8 * h < tail ? vs[h] * v_ref : 1.0f;
+              near = near && vs[h] >= 0x1p-10f && vs[h] <= 0x1p6f;
+            }
+            near = __all_sync(0xffffffffu, near);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)  // (a hidden key's scale may be a NaN, which is not near)
+                s[nb][e] = !near && s[nb][e] == 0.0f ? 0.0f : s[nb][e] * vs[e >> 1];
+            auto add = [&](auto half_type, auto clear) {
+              using P = decltype(half_type);
+              constexpr bool kBf = std::is_same<P, __nv_bfloat16>::value;
+              uint32_t pf[NB][2];
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (P*)nullptr));
+#pragma unroll
+              for (int k = 0; k < DT; k += 2) {
+                uint32_t b[4];  // units k and k + 1, each keys 0-7 and 8-15
+                ldsm_x4_t(b, ldsm_at(vbase, k / 2));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  // codes of two keys: even columns (rows 0-7 of the 16-wide
+                  // side) together, and odd ones
+                  uint32_t f[4];
+                  e4m3_to_half(__byte_perm(b[2 * u], 0, 0x3120), f[0], f[1]);
+                  e4m3_to_half(__byte_perm(b[2 * u + 1], 0, 0x3120), f[2], f[3]);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    if constexpr (kBf) f[e] = half2_to_bf16(f[e]);
+                    if constexpr (decltype(clear)::value) f[e] &= keep(e >> 1);
+                  }
+#pragma unroll
+                  for (int nb = 0; nb < NB; ++nb) mma16<kBf>(o[k + u][nb], f, pf[nb][0], pf[nb][1]);
+                }
+              }
+            };
+            if (!near) add(__nv_bfloat16(), std::true_type());
+            else if (tail < 16) add(__half(), std::true_type());
+            else add(__half(), std::false_type());
+          }
         }
+        strip -= KEYS / 16;
+        if (flags & kEnds) break;
+        release();
+        next_tile();
+        if (!ok) break;
       }
-      strip -= KEYS / 16;
-
-      if (flags & kEnds) {
-        // ---- join the warps
-        constexpr int ROWS = Cfg::ROWS, SLOTS = Cfg::SLOTS;
+      if (!ok) break;
+      {
+        const TileInfo& info = infos[st];
+        // ---- join the warps: maxima and sums, then SLOTS warps' rows at a
+        // time through the place of the ring whose tile was the piece's last
+        // (nobody reads it any more once all have met), added in the warps'
+        // order.  The maxima and sums of two pieces alternate between two
+        // places: a warp may be one piece ahead of another, not two.
+        constexpr int ROWS = Cfg::ROWS, SLOTS = Cfg::SLOTS, RPW = (ROWS + WARPS - 1) / WARPS;
+        float2* mls = ml + piece * WARPS * ROWS;
+        piece ^= 1;
+        float* slots = reinterpret_cast<float*>(ring + size_t(st) * 2 * HALF);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], x);
-            if (g == 0) ml[warp * ROWS + 8 * nb + 2 * t + e] = make_float2(m[nb][e], l[nb][e]);
+            if (g == 0) mls[warp * ROWS + 8 * nb + 2 * t + e] = make_float2(m[nb][e], l[nb][e]);
           }
         meet();
-        auto total_of = [&](int r) -> float2 {
-          float mt = kNone, lt = 0.0f;
-#pragma unroll
-          for (int x = 0; x < WARPS; ++x) {
-            const float2 y = ml[x * ROWS + r];
-            if (y.y != 0.0f) mt = fmaxf(mt, y.x);
-          }
-#pragma unroll
-          for (int x = 0; x < WARPS; ++x) {
-            const float2 y = ml[x * ROWS + r];
-            if (y.y != 0.0f) lt += y.y * ex2_approx(y.x - mt);
-          }
-          return make_float2(mt, lt);
-        };
         const float v_up = Q8 && v_ref != 0.0f ? 1.0f / v_ref : 1.0f;
-        // the warps add their rows, SLOTS at a time, always in the same order
-        float* mine = merge + (warp % SLOTS) * ROWS * D;
+        float2 tot[RPW];   // of the rows this warp writes: warp, warp + WARPS, ...
+        float acc[RPW][D / 32];
+#pragma unroll
+        for (int y = 0; y < RPW; ++y) {
+          tot[y] = make_float2(kNone, 0.0f);
+          const int r = min(warp + y * WARPS, ROWS - 1);
+#pragma unroll
+          for (int x = 0; x < WARPS; ++x) {
+            const float2 z = mls[x * ROWS + r];
+            if (z.y != 0.0f) tot[y].x = fmaxf(tot[y].x, z.x);
+          }
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) acc[y][c] = 0.0f;
+        }
 #pragma unroll 1
-        for (int pass = 0; pass < (WARPS + SLOTS - 1) / SLOTS; ++pass) {
-          if (warp / SLOTS == pass) {
+        for (int pass = 0; pass < WARPS; pass += SLOTS) {
+          if (warp >= pass && warp < pass + SLOTS) {
+            float* mine = slots + (warp - pass) * ROWS * D;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int r = 8 * nb + 2 * t + e;
-                const float f = ex2_approx(m[nb][e] - total_of(r).x) * v_up;
+              for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int k = 0; k < DT; ++k)
 #pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    float* at = mine + merge_at<D>(r, 16 * k + (Q8 ? 2 * g + h : g + 8 * h));
-                    // a warp that saw no key leaves zeros, whatever 0 * its sums is
-                    const float x = l[nb][e] == 0.0f ? 0.0f : o[k][nb][e + 2 * h] * f;
-                    *at = pass == 0 ? x : *at + x;
-                  }
-              }
+                  for (int h = 0; h < 2; ++h)
+                    mine[merge_at<D>(8 * nb + 2 * t + e, 16 * k + (Q8 ? 2 * g + h : g + 8 * h))] =
+                        o[k][nb][e + 2 * h] * v_up;
           }
           meet();
+#pragma unroll
+          for (int y = 0; y < RPW; ++y) {
+            const int r = min(warp + y * WARPS, ROWS - 1);
+#pragma unroll
+            for (int x = 0; x < SLOTS; ++x) {
+              if (pass + x >= WARPS) break;
+              const float2 z = mls[(pass + x) * ROWS + r];
+              if (z.y == 0.0f) continue;  // saw no key: its sums are 0 times what may be anything
+              const float f = ex2_approx(z.x - tot[y].x);
+              tot[y].y = fmaf(z.y, f, tot[y].y);
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c)
+                acc[y][c] = fmaf(slots[x * ROWS * D + merge_at<D>(r, lane + 32 * c)], f, acc[y][c]);
+            }
+          }
+          if (pass + SLOTS < WARPS) meet();
         }
         // ---- write out, a warp a row
-#pragma unroll 1
-        for (int r = warp; r < ROWS; r += WARPS) {
+#pragma unroll
+        for (int y = 0; y < RPW; ++y) {
+          const int r = warp + y * WARPS;
+          if (r >= ROWS || !ok) continue;
           const Row row = row_of(p, info, r);
-          const float2 tot = total_of(r);
           bool bad = false;
 #pragma unroll
-          for (int d = lane; d < D; d += 32) {
-            float* at = merge + merge_at<D>(r, d);
-            float x = 0.0f;
-#pragma unroll
-            for (int y = 0; y < SLOTS; ++y) x += at[y * ROWS * D];
-            bad = bad || (__float_as_uint(x) & 0x7fffffffu) >= 0x7f800000u;
-            at[0] = x;
+          for (int c = 0; c < D / 32; ++c) bad = bad || (__float_as_uint(acc[y][c]) & 0x7fffffffu) >= 0x7f800000u;
+          if (!row.valid) continue;
+          if (__any_sync(0xffffffffu, bad) && tot[y].y > 0.0f && tot[y].y <= 3.4028234663852886e38f) {
+            const T* q = static_cast<const T*>(p.Q) + int64_t(info.q0 + row.token) * p.q_token + row.head * p.q_head;
+            redo_row<T, D, Q8>(p, info.b, info.k0, info.hk, q, info.piece_key, min(row.lim, info.key + KEYS), tot[y].x,
+                               acc[y]);
           }
-          bad = __any_sync(0xffffffffu, bad) && row.valid && tot.y > 0.0f && tot.y <= 3.4028234663852886e38f;
-          const T* q = static_cast<const T*>(p.Q) + int64_t(info.q0 + row.token) * p.q_token + row.head * p.q_head;
-          if (ok && bad)
-            redo_row<T, D, Q8>(p, info.b, info.k0, info.hk, q, info.piece_key, min(row.lim, info.key + KEYS), tot.x,
-                               merge, r);
-          __syncwarp();
-          if (!ok || !row.valid) continue;
           if (flags & kWhole) {
-            const float inv = tot.y == 0.0f ? 0.0f : 1.0f / tot.y;
-            T* out = static_cast<T*>(p.O) + int64_t(info.q0 + row.token) * p.o_token + row.head * p.o_head;
-            for (int d = lane; d < D; d += 32) stf(out + d, tot.y == 0.0f ? 0.0f : merge[merge_at<D>(r, d)] * inv);
+            const float inv = tot[y].y == 0.0f ? 0.0f : 1.0f / tot[y].y;
+            T* out = static_cast<T*>(p.O) + int64_t(info.q0 + row.token) * p.o_token + row.head * p.o_head + lane;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) stf(out + 32 * c, tot[y].y == 0.0f ? 0.0f : acc[y][c] * inv);
           } else {
             // a piece of a unit that began in an earlier block goes to the
             // first place, one that goes on in the next block to the second
             const int64_t at = (int64_t(blockIdx.x) * 2 + (flags & kFirst ? 1 : 0)) * ROWS + r;
-            if (lane == 0) a.part_ml[at] = tot;
-            for (int d = lane; d < D; d += 32) a.part_o[at * D + d] = merge[merge_at<D>(r, d)];
+            if (lane == 0) a.part_ml[at] = tot[y];
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) a.part_o[at * D + lane + 32 * c] = acc[y][c];
           }
         }
-        meet();  // the merge area is free again
+        fence_proxy_async_smem();  // before TMA writes the place again
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
-      if (++st == STAGES) {
-        st = 0;
-        phase ^= 1u;
-      }
+      release();
     }
     if (!ok && lane == 0) rec_err(a.err, abort_flag, kDevTimeoutFull);
+  }
+  // rows outside every sequence (else the joining kernel's)
+  if (p.zero_rest && a.whole) {
+    const int2 rest = seq_rest(p);
+    const int64_t row_len = int64_t(p.heads_q) * D;
+    for (int tok = blockIdx.x; tok < p.tokens_q; tok += gridDim.x)
+      if (tok < rest.x || tok >= rest.y)
+        for (int i = threadIdx.x; i < row_len; i += THREADS)
+          stf(static_cast<T*>(p.O) + int64_t(tok) * p.o_token + (i / D) * p.o_head + i % D, 0.0f);
   }
 }
 
@@ -877,30 +939,40 @@ __global__ void __launch_bounds__(128) attention_decode_combine(const DecodePara
   const int hk = h / p.group, q = (t - s.q0) * p.group + h - hk * p.group;
   const int nt = unit_tiles(a, s.len), nrt = row_tiles(a, s.n);
   const int total = a.plan[p.batch], used = a.plan[p.batch + 1];
-  const int first = a.plan[b] + (hk * nrt + q / a.rows) * nt;
-  // block that holds a tile: the last c with c * total / used <= tile
+  // the first tile's last place; the others follow
+  const int first = a.plan[b] + (hk * nrt + q / a.rows) * unit_weight(a, nt) + kUnitCost;
+  // block that holds a place: the last c with c * total / used <= place
   const int c0 = min(int((int64_t(first + 1) * used - 1) / total), used - 1);
   const int c1 = min(int((int64_t(first + nt) * used - 1) / total), used - 1);
   if (c0 >= c1) return;  // whole in one block: written there
-  auto at = [&](int c) -> int64_t { return (int64_t(c) * 2 + (first_tile(c, total, used) <= first ? 1 : 0)) * a.rows + q % a.rows; };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) {
-    const float2 ml = a.part_ml[at(c)];
-    if (ml.y != 0.0f) m = fmaxf(m, ml.x);
-  }
-#pragma unroll
-  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
-  float l = 0.0f, o[N];
+  auto at = [&](int c) -> int64_t { return (int64_t(c) * 2 + (first_place(c, total, used) <= first ? 1 : 0)) * a.rows + q % a.rows; };
+  // 32 pieces at a time, a lane each; their rows are then independent loads
+  float m = kNone, l = 0.0f, o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.0f;
-  for (int c = c0; c <= c1; ++c) {
-    const int64_t x = at(c);
-    const float2 ml = a.part_ml[x];
-    if (ml.y == 0.0f) continue;
-    const float wgt = ex2_approx(ml.x - m);
-    l = fmaf(wgt, ml.y, l);
+  for (int base = c0; base <= c1; base += 32) {
+    const int64_t mine = base + lane <= c1 ? at(base + lane) : -1;
+    const float2 ml = mine >= 0 ? a.part_ml[mine] : make_float2(kNone, 0.0f);
+    float top = ml.y != 0.0f ? ml.x : kNone;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = fmaf(wgt, a.part_o[x * D + lane * N + i], o[i]);
+    for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    const float m_new = fmaxf(m, top), old = ex2_approx(m - m_new);
+    const float wgt = ml.y != 0.0f ? ex2_approx(ml.x - m_new) : 0.0f;
+    float sum = wgt * ml.y;
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    l = fmaf(l, old, sum);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] *= old;
+    m = m_new;
+    const int n = min(32, c1 - base + 1);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float f = __shfl_sync(0xffffffffu, wgt, k);
+      const float* src = a.part_o + __shfl_sync(0xffffffffu, mine, k) * D + lane * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = fmaf(f, src[i], o[i]);  // (a piece that saw no key holds zeros)
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -913,6 +985,9 @@ int decode_keys(const SeqProblem& p, bool q8) {
                    : (q8 ? DecodeCfg<128, true, 1>::KEYS : DecodeCfg<128, false, 1>::KEYS);
 }
 int64_t decode_blocks(const DeviceInfo& dev, int rows) { return int64_t(dev.num_sms) * (rows == 8 ? 2 : 1); }
+// Sequences that cannot be long: splitting them among blocks would save less
+// than the second kernel costs.
+bool decode_whole(const SeqProblem& p) { return (p.table != nullptr ? p.max_keys : p.tokens_kv) <= 512; }
 
 template <int FMT, int D, bool Q8, int NB>
 cudaError_t launch_decode_rows(const DecodeParams& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
@@ -933,7 +1008,7 @@ cudaError_t launch_decode_rows(const DecodeParams& a, const CUtensorMap& tk, con
   cudaLaunchAttribute attr[1];
   apply_pdl(cfg, attr, 0);
   e = cudaLaunchKernelEx(&cfg, kern, tk, tv, a);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || a.whole) return e;
   cfg.gridDim = dim3(unsigned((int64_t(a.p.tokens_q) * a.p.heads_q + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
@@ -961,6 +1036,7 @@ bool seq_decode_ok(const SeqProblem& p, int dtype, int kv_dtype) {
 }
 
 size_t seq_decode_workspace(const SeqProblem& p, int rows, const DeviceInfo& dev) {
+  if (decode_whole(p)) return 0;
   return size_t(decode_blocks(dev, rows)) * 2 * size_t(rows) * (size_t(p.d) * 4 + 8) + (size_t(p.batch) + 2) * 4;
 }
 
@@ -972,11 +1048,18 @@ cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, int 
   a.rows = rows;
   a.keys = decode_keys(p, q8);
   a.box_rows = paged && p.page_size < a.keys ? p.page_size : a.keys;
-  a.blocks = int(decode_blocks(dev, rows));
-  a.min_tiles = 1;
-  a.part_o = static_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(a.blocks) * 2 * rows * p.d);
-  a.plan = reinterpret_cast<int*>(a.part_ml + int64_t(a.blocks) * 2 * rows);
+  a.whole = decode_whole(p);
+  if (a.whole) {
+    // a block a unit, up to a few waves
+    const int64_t units = ((int64_t(p.tokens_q) * p.group + int64_t(p.batch) * (rows - 1)) / rows) * p.heads_kv;
+    const int64_t most = 8 * decode_blocks(dev, rows);
+    a.blocks = int(units < 1 ? 1 : units < most ? units : most);
+  } else {
+    a.blocks = int(decode_blocks(dev, rows));
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(a.blocks) * 2 * rows * p.d);
+    a.plan = reinterpret_cast<int*>(a.part_ml + int64_t(a.blocks) * 2 * rows);
+  }
   a.err = err;
   CUtensorMap tk, tv;
   if (!seq_kv_maps(p, kv_dtype, a.box_rows, true, &tk, &tv)) return cudaErrorInvalidValue;

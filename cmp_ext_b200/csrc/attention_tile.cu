@@ -751,22 +751,33 @@ __global__ void __launch_bounds__(128) attention_seq_combine(const SeqProblem p,
   if (t < rest.x || t >= rest.y) {
     if (!p.zero_rest) return;
   } else {
-    float m = -INFINITY;
-    for (int z = lane; z < splits; z += 32) {
-      const float2 ml = part_ml[z * rows + row];
-      if (ml.y != 0.0f) m = fmaxf(m, ml.x);
-    }
+    // 32 splits at a time, a lane each; their rows are then independent loads
+    float m = -INFINITY, l = 0.0f;
+    for (int base = 0; base < splits; base += 32) {
+      const float2 ml = base + lane < splits ? part_ml[(base + lane) * rows + row] : make_float2(-INFINITY, 0.0f);
+      float top = ml.y != 0.0f ? ml.x : -INFINITY;
 #pragma unroll
-    for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
-    float l = 0.0f;
-    for (int z = 0; z < splits; ++z) {
-      const float2 ml = part_ml[z * rows + row];
-      if (ml.y == 0.0f) continue;
-      const float w = ex2_approx(ml.x - m);
-      l = fmaf(w, ml.y, l);
-      const float* src = part_o + (z * rows + row) * D + lane * N;
+      for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+      const float m_new = fmaxf(m, top);
+      const float old = l == 0.0f ? 0.0f : ex2_approx(m - m_new);
+      const float wgt = ml.y != 0.0f ? ex2_approx(ml.x - m_new) : 0.0f;
+      float sum = wgt * ml.y;
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = fmaf(w, src[i], o[i]);
+      for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+      l = fmaf(l, old, sum);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] *= old;
+      m = m_new;
+      const unsigned there = __ballot_sync(0xffffffffu, ml.y != 0.0f);  // the others left no row
+      const int n = min(32, splits - base);
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float f = __shfl_sync(0xffffffffu, wgt, k);
+        if (!(there >> k & 1)) continue;
+        const float* src = part_o + ((base + k) * rows + row) * D + lane * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fmaf(f, src[i], o[i]);
+      }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
