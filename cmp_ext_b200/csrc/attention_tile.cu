@@ -422,6 +422,32 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
       const int n[2] = {n0, n1};
       int qk[2] = {0, 0}, pv[2] = {0, 0};  // products issued
       int k_rel = 0, v_rel = 0;            // key / value blocks released
+      // S = Q K^T of tile t's next block, if its keys are there.  The tile's
+      // last P V must be done: P lies where S goes.
+      auto issue_qk = [&](int t) -> bool {
+        const int j = qk[t];
+        if (!mbar_test_wait(&k_full[j % KS], (j / KS) & 1)) return false;
+        tc_fence_after();
+        const uint32_t q_addr = smem_u32(sQ + t * Cfg::TILE);
+        const uint32_t k_addr = smem_u32(sK + (j % KS) * Cfg::TILE);
+#pragma unroll
+        for (int c = 0; c < Cfg::QCH; ++c)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f16(tmem_base + uint32_t(t * 128), make_sdesc_sw128(q_addr + c * 16384 + kk * 32, 16, 1024),
+                    make_sdesc_sw128(k_addr + c * 16384 + kk * 32, 16, 1024), IDESC_QK, (c | kk) != 0 ? 1u : 0u);
+        mma_commit(&s_full[t]);
+        ++qk[t];
+        while (k_rel < nkv && (qk[0] > k_rel || n0 <= k_rel) && (qk[1] > k_rel || n1 <= k_rel)) {
+          mma_commit(&k_empty[k_rel % KS]);
+          ++k_rel;
+        }
+        return true;
+      };
+      // A tile's P V and next Q K^T go out together, so that the two tiles
+      // fall out of step: one is in softmax while the other's products run
+      // (issued as they became ready, both tiles' softmax ran at once and the
+      // tensor core waited: 5500 cycles a block of both, now NNNN).
       uint32_t idle = 0;  // polls since the last product
       uint64_t t0 = 0;
       while (ok && (pv[0] < n0 || pv[1] < n1)) {
@@ -429,46 +455,34 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (qk[t] == pv[t]) {
-            // S of block j: the last product of this tile must be done with
-            // P, which lies where S goes
-            const int j = qk[t];
-            if (j < n[t] && mbar_test_wait(&k_full[j % KS], (j / KS) & 1) &&
-                (j == 0 || mbar_test_wait(&o_done[t], (j - 1) & 1))) {
-              tc_fence_after();
-              const uint32_t q_addr = smem_u32(sQ + t * Cfg::TILE);
-              const uint32_t k_addr = smem_u32(sK + (j % KS) * Cfg::TILE);
+            if (qk[t] < n[t]) any = issue_qk(t) || any;
+            continue;
+          }
+          const int j = pv[t];
+          const bool cleared = Q8 || j + 1 < nkv || last_keys == 128 || mbar_test_wait(tail, 0);
+          if (!cleared || !mbar_test_wait(&p_full[t], j & 1) || !mbar_test_wait(&v_full[j % VS], (j / VS) & 1)) continue;
+          tc_fence_after();
+          const uint32_t v_addr = smem_u32(sV + (j % VS) * Cfg::TILE);
+          const int steps = j + 1 < nkv ? 8 : (last_keys + 15) >> 4;
 #pragma unroll
-              for (int c = 0; c < Cfg::QCH; ++c)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                  mma_f16(tmem_base + uint32_t(t * 128), make_sdesc_sw128(q_addr + c * 16384 + kk * 32, 16, 1024),
-                          make_sdesc_sw128(k_addr + c * 16384 + kk * 32, 16, 1024), IDESC_QK, (c | kk) != 0 ? 1u : 0u);
-              mma_commit(&s_full[t]);
-              ++qk[t];
-              any = true;
-              while (k_rel < nkv && (qk[0] > k_rel || n0 <= k_rel) && (qk[1] > k_rel || n1 <= k_rel)) {
-                mma_commit(&k_empty[k_rel % KS]);
-                ++k_rel;
-              }
+          for (int kk = 0; kk < 8; ++kk)
+            if (kk < steps)
+              mma_f16_ts(tmem_base + 256u + uint32_t(t * D), tmem_base + uint32_t(t * 128 + kk * 8),
+                         make_sdesc_sw128(v_addr + kk * 2048, 16384, 1024), IDESC_PV, (j | kk) != 0 ? 1u : 0u);
+          mma_commit(&o_done[t]);
+          ++pv[t];
+          any = true;
+          while (v_rel < nkv && (pv[0] > v_rel || n0 <= v_rel) && (pv[1] > v_rel || n1 <= v_rel)) {
+            mma_commit(&v_empty[v_rel % VS]);
+            ++v_rel;
+          }
+          if (qk[t] < n[t]) {
+            if (!mbar_wait(&o_done[t], j & 1, abort_flag)) {
+              rec_err(a.err, abort_flag, kDevTimeoutFull);
+              ok = false;
+              break;
             }
-          } else {
-            const int j = pv[t];
-            const bool cleared = Q8 || j + 1 < nkv || last_keys == 128 || mbar_test_wait(tail, 0);
-            if (cleared && mbar_test_wait(&v_full[j % VS], (j / VS) & 1) && mbar_test_wait(&p_full[t], j & 1)) {
-              tc_fence_after();
-              const uint32_t v_addr = smem_u32(sV + (j % VS) * Cfg::TILE);
-              const int steps = j + 1 < nkv ? 8 : (last_keys + 15) >> 4;
-              for (int kk = 0; kk < steps; ++kk)
-                mma_f16_ts(tmem_base + 256u + uint32_t(t * D), tmem_base + uint32_t(t * 128 + kk * 8),
-                           make_sdesc_sw128(v_addr + kk * 2048, 16384, 1024), IDESC_PV, (j | kk) != 0 ? 1u : 0u);
-              mma_commit(&o_done[t]);
-              ++pv[t];
-              any = true;
-              while (v_rel < nkv && (pv[0] > v_rel || n0 <= v_rel) && (pv[1] > v_rel || n1 <= v_rel)) {
-                mma_commit(&v_empty[v_rel % VS]);
-                ++v_rel;
-              }
-            }
+            issue_qk(t);
           }
         }
         idle = any ? 0 : idle + 1;
