@@ -416,8 +416,16 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    if (lane == 0 && nkv > 0) {
-      bool ok = mbar_wait(q_full, 0, abort_flag);
+    // the whole warp walks along, one lane issues
+    if (nkv > 0) {
+      const uint32_t one = elect_one();
+      auto ready = [&](uint64_t* bar, int phase) -> bool {
+        return __all_sync(0xffffffffu, mbar_test_wait(bar, uint32_t(phase & 1)));
+      };
+      auto wait = [&](uint64_t* bar, int phase) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bar, uint32_t(phase & 1), abort_flag));
+      };
+      bool ok = wait(q_full, 0);
       if (!ok) rec_err(a.err, abort_flag, kDevTimeoutFull);
       const int n[2] = {n0, n1};
       int qk[2] = {0, 0}, pv[2] = {0, 0};  // products issued
@@ -426,7 +434,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
       // last P V must be done: P lies where S goes.
       auto issue_qk = [&](int t) -> bool {
         const int j = qk[t];
-        if (!mbar_test_wait(&k_full[j % KS], (j / KS) & 1)) return false;
+        if (!ready(&k_full[j % KS], j / KS)) return false;
         tc_fence_after();
         const uint32_t q_addr = smem_u32(sQ + t * Cfg::TILE);
         const uint32_t k_addr = smem_u32(sK + (j % KS) * Cfg::TILE);
@@ -434,12 +442,12 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
         for (int c = 0; c < Cfg::QCH; ++c)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_f16(tmem_base + uint32_t(t * 128), make_sdesc_sw128(q_addr + c * 16384 + kk * 32, 16, 1024),
+            mma_f16_one(one, tmem_base + uint32_t(t * 128), make_sdesc_sw128(q_addr + c * 16384 + kk * 32, 16, 1024),
                     make_sdesc_sw128(k_addr + c * 16384 + kk * 32, 16, 1024), IDESC_QK, (c | kk) != 0 ? 1u : 0u);
-        mma_commit(&s_full[t]);
+        mma_commit_one(one, &s_full[t]);
         ++qk[t];
         while (k_rel < nkv && (qk[0] > k_rel || n0 <= k_rel) && (qk[1] > k_rel || n1 <= k_rel)) {
-          mma_commit(&k_empty[k_rel % KS]);
+          mma_commit_one(one, &k_empty[k_rel % KS]);
           ++k_rel;
         }
         return true;
@@ -459,25 +467,25 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
             continue;
           }
           const int j = pv[t];
-          const bool cleared = Q8 || j + 1 < nkv || last_keys == 128 || mbar_test_wait(tail, 0);
-          if (!cleared || !mbar_test_wait(&p_full[t], j & 1) || !mbar_test_wait(&v_full[j % VS], (j / VS) & 1)) continue;
+          const bool cleared = Q8 || j + 1 < nkv || last_keys == 128 || ready(tail, 0);
+          if (!cleared || !ready(&p_full[t], j) || !ready(&v_full[j % VS], j / VS)) continue;
           tc_fence_after();
           const uint32_t v_addr = smem_u32(sV + (j % VS) * Cfg::TILE);
           const int steps = j + 1 < nkv ? 8 : (last_keys + 15) >> 4;
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
             if (kk < steps)
-              mma_f16_ts(tmem_base + 256u + uint32_t(t * D), tmem_base + uint32_t(t * 128 + kk * 8),
+              mma_f16_ts_one(one, tmem_base + 256u + uint32_t(t * D), tmem_base + uint32_t(t * 128 + kk * 8),
                          make_sdesc_sw128(v_addr + kk * 2048, 16384, 1024), IDESC_PV, (j | kk) != 0 ? 1u : 0u);
-          mma_commit(&o_done[t]);
+          mma_commit_one(one, &o_done[t]);
           ++pv[t];
           any = true;
           while (v_rel < nkv && (pv[0] > v_rel || n0 <= v_rel) && (pv[1] > v_rel || n1 <= v_rel)) {
-            mma_commit(&v_empty[v_rel % VS]);
+            mma_commit_one(one, &v_empty[v_rel % VS]);
             ++v_rel;
           }
           if (qk[t] < n[t]) {
-            if (!mbar_wait(&o_done[t], j & 1, abort_flag)) {
+            if (!wait(&o_done[t], j)) {
               rec_err(a.err, abort_flag, kDevTimeoutFull);
               ok = false;
               break;
@@ -488,19 +496,19 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
         idle = any ? 0 : idle + 1;
         if ((idle & 1023u) == 1023u) {
           if (idle == 1023u) t0 = globaltimer_ns();
-          else if (*abort_flag || globaltimer_ns() - t0 > CMPX_WAIT_TIMEOUT_NS) {
+          else if (__any_sync(0xffffffffu, *abort_flag || globaltimer_ns() - t0 > CMPX_WAIT_TIMEOUT_NS)) {
             rec_err(a.err, abort_flag, kDevTimeoutFull);
             ok = false;
           }
         }
       }
       // the last commits reach their barriers before the block may exit
-      if (ok && !mbar_wait(&v_empty[(nkv - 1) % VS], ((nkv - 1) / VS) & 1, abort_flag)) {
+      if (ok && !wait(&v_empty[(nkv - 1) % VS], (nkv - 1) / VS)) {
         rec_err(a.err, abort_flag, kDevTimeoutFull);
         ok = false;
       }
       if (!ok) {
-        mma_commit(drain);
+        mma_commit_one(one, drain);
         volatile int never = 0;
         mbar_wait(drain, 0, &never);
       }
