@@ -69,7 +69,7 @@ struct DecodeParams {
   int keys;         // of a tile
   float* part_o;    // [blocks][2][rows][D]
   float2* part_ml;  // [blocks][2][rows]
-  int* plan;        // [batch + 2]: tiles before each sequence, their number, blocks in use
+  int* joints;      // [tokens_q][heads_q]: first block, pieces << 12, row of the unit << 24 (one piece: written)
   int* err;
 };
 
@@ -145,8 +145,8 @@ struct Walk {
     nrt = row_tiles(a, s.n);
     nt = unit_tiles(a, s.len);
   }
-  // The tile at place `rel` of sequence `seq`.
-  __device__ __forceinline__ void at(const DecodeParams& a, int seq, int rel) {
+  // The tile at place `rel` of sequence `seq`; returns the place in its unit.
+  __device__ __forceinline__ int at(const DecodeParams& a, int seq, int rel) {
     b = seq;
     enter(a);
     const int weight = unit_weight(a, nt), per_head = nrt * weight;
@@ -154,6 +154,7 @@ struct Walk {
     rel -= hk * per_head;
     rt = rel / weight;
     j = place_tile(a, rel - rt * weight);
+    return rel - rt * weight;
   }
   __device__ __forceinline__ void next_unit(const DecodeParams& a) {
     j = 0;
@@ -180,7 +181,8 @@ struct alignas(16) TileInfo {
   int piece_key;     // first key of the piece of the unit that this block has
   int b, hk, row0;   // sequence, kv head, first query row (token x head of the group)
   int q0, n, k0;     // of Seq
-  int pad[2];
+  int pieces;        // blocks that have one, counted from this block
+  int pad;
 };
 constexpr int kEnds = 1;     // the piece's last tile
 constexpr int kWhole = 2;    // the piece is the whole unit
@@ -340,14 +342,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
   int total = 0;
   for (int base = 0; base < p.batch; base += THREADS) {
     const int all = count_pass(base);
-    if (blockIdx.x == 0 && !a.whole && base + int(threadIdx.x) < p.batch) a.plan[base + threadIdx.x] = total + upto - mine;
     total += all;
   }
   const int used = min(total, a.blocks);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && !a.whole) {
-    a.plan[p.batch] = total;
-    a.plan[p.batch + 1] = used;
-  }
   // the places of its first tile and of the next block's
   const int c_id = int(blockIdx.x);
   const int lo = c_id < used ? first_place(c_id, total, used) : 0;
@@ -369,8 +366,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
   __syncthreads();
   bool busy = lo < hi;
   Walk w = {}, end = {};
+  int unit0 = 0;  // the unit's first place
   if (busy) {
-    w.at(a, start[0], start[1]);
+    unit0 = lo - w.at(a, start[0], start[1]);
     end.b = p.batch;
     if (hi < total) end.at(a, start[2], start[3]);
     busy = !w.is(end);
@@ -434,9 +432,20 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       info.k0 = k0;
       const int boxes = min(boxes_full, (w.s.len - kv0 + a.box_rows - 1) / a.box_rows);
       const bool unit_ends = w.j + 1 == w.nt;
-      if (unit_ends) w.next_unit(a);
-      else ++w.j;
+      const int unit_end = unit0 + unit_weight(a, w.nt);
+      if (unit_ends) {
+        w.next_unit(a);
+        unit0 = unit_end;
+      } else {
+        ++w.j;
+      }
       last = w.is(end) || w.b >= p.batch;
+      // blocks that hold a piece of the unit, where this is not its last tile:
+      // up to the one that holds its last place, the last c with
+      // c * total / used <= place
+      info.pieces = 1;
+      if (last && !unit_ends)
+        info.pieces = min(int((int64_t(unit_end) * used - 1) / total), used - 1) - int(blockIdx.x) + 1;
       info.flags = (unit_ends || last ? kEnds : 0) | (piece_key == 0 ? kFirst : 0) |
                    (piece_key == 0 && unit_ends ? kWhole : 0) | (last ? kLast : 0);
       begins = unit_ends;
@@ -867,6 +876,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) bad = bad || (__float_as_uint(acc[y][c]) & 0x7fffffffu) >= 0x7f800000u;
           if (!row.valid) continue;
+          // the unit's first block says where its pieces lie
+          if (!a.whole && (flags & kFirst) && lane == 0)
+            a.joints[int64_t(info.q0 + row.token) * p.heads_q + row.head] =
+                int(blockIdx.x) | info.pieces << 12 | r << 24;
           if (__any_sync(0xffffffffu, bad) && tot[y].y > 0.0f && tot[y].y <= 3.4028234663852886e38f) {
             const T* q = static_cast<const T*>(p.Q) + int64_t(info.q0 + row.token) * p.q_token + row.head * p.q_head;
             redo_row<T, D, Q8>(p, info.b, info.k0, info.hk, q, info.piece_key, min(row.lim, info.key + KEYS), tot[y].x,
@@ -922,30 +935,13 @@ __global__ void __launch_bounds__(128) attention_decode_combine(const DecodePara
       for (int i = 0; i < N; ++i) stf(out + i, 0.0f);
     return;
   }
-  int b;
-  if (p.cu_q == nullptr) {
-    b = t / p.uniform_n;
-  } else {
-    int lo = 0, hi = p.batch;  // first sequence that begins behind t
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(p.cu_q + mid) <= t) lo = mid + 1; else hi = mid;
-    }
-    b = lo - 1;
-  }
-  if (b < 0 || b >= p.batch) return;
-  const Seq s = seq_of(p, b);
-  if (t < s.q0 || t >= s.q0 + s.n) return;
-  const int hk = h / p.group, q = (t - s.q0) * p.group + h - hk * p.group;
-  const int nt = unit_tiles(a, s.len), nrt = row_tiles(a, s.n);
-  const int total = a.plan[p.batch], used = a.plan[p.batch + 1];
-  // the first tile's last place; the others follow
-  const int first = a.plan[b] + (hk * nrt + q / a.rows) * unit_weight(a, nt) + kUnitCost;
-  // block that holds a place: the last c with c * total / used <= place
-  const int c0 = min(int((int64_t(first + 1) * used - 1) / total), used - 1);
-  const int c1 = min(int((int64_t(first + nt) * used - 1) / total), used - 1);
+  // (clamped: offsets that are not ascending leave rows that no block wrote)
+  const int joint = a.joints[row];
+  const int c0 = min(joint & 0xfff, a.blocks - 1), c1 = min(c0 + (joint >> 12 & 0xfff) - 1, a.blocks - 1);
+  const int r = min(joint >> 24 & 0xff, a.rows - 1);
   if (c0 >= c1) return;  // whole in one block: written there
-  auto at = [&](int c) -> int64_t { return (int64_t(c) * 2 + (first_place(c, total, used) <= first ? 1 : 0)) * a.rows + q % a.rows; };
+  // the unit begins in block c0's second piece and goes on in the others' first
+  auto at = [&](int c) -> int64_t { return (int64_t(c) * 2 + (c == c0 ? 1 : 0)) * a.rows + r; };
   // 32 pieces at a time, a lane each; their rows are then independent loads
   float m = kNone, l = 0.0f, o[N];
 #pragma unroll
@@ -1037,7 +1033,7 @@ bool seq_decode_ok(const SeqProblem& p, int dtype, int kv_dtype) {
 
 size_t seq_decode_workspace(const SeqProblem& p, int rows, const DeviceInfo& dev) {
   if (decode_whole(p)) return 0;
-  return size_t(decode_blocks(dev, rows)) * 2 * size_t(rows) * (size_t(p.d) * 4 + 8) + (size_t(p.batch) + 2) * 4;
+  return size_t(decode_blocks(dev, rows)) * 2 * size_t(rows) * (size_t(p.d) * 4 + 8) + size_t(p.tokens_q) * size_t(p.heads_q) * 4;
 }
 
 cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, int rows, void* ws, const DeviceInfo& dev,
@@ -1058,7 +1054,7 @@ cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, int 
     a.blocks = int(decode_blocks(dev, rows));
     a.part_o = static_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(a.blocks) * 2 * rows * p.d);
-    a.plan = reinterpret_cast<int*>(a.part_ml + int64_t(a.blocks) * 2 * rows);
+    a.joints = reinterpret_cast<int*>(a.part_ml + int64_t(a.blocks) * 2 * rows);
   }
   a.err = err;
   CUtensorMap tk, tv;

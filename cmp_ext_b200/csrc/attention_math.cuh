@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 
 #include <cstdint>
 
@@ -79,5 +80,21 @@ __device__ __forceinline__ float e8m0_to_float(uint32_t b) {
 __device__ __forceinline__ void stf(float* p, float v) { *p = v; }
 __device__ __forceinline__ void stf(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void stf(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Two e4m3 codes times a scale, in T, saturating.
+__device__ __forceinline__ uint32_t dequant2(uint32_t codes, float up, __half*) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y * up), "f"(f.x * up));
+  return r;
+}
+__device__ __forceinline__ uint32_t dequant2(uint32_t codes, float up, __nv_bfloat16*) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  uint32_t r;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y * up), "f"(f.x * up));
+  return r;
+}
 
 }  // namespace cmpx

@@ -93,22 +93,6 @@ __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// Two e4m3 codes times a scale, in T, saturating.
-__device__ __forceinline__ uint32_t dequant2(uint32_t codes, float up, __half*) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3);
-  const float2 f = __half22float2(__half2(h));
-  uint32_t r;
-  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y * up), "f"(f.x * up));
-  return r;
-}
-__device__ __forceinline__ uint32_t dequant2(uint32_t codes, float up, __nv_bfloat16*) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3);
-  const float2 f = __half22float2(__half2(h));
-  uint32_t r;
-  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y * up), "f"(f.x * up));
-  return r;
-}
-
 // One row from its definition: keys [kbeg, kend) of sequence s / head hk,
 // weights 2^(x - m).  A warp computes it, lane d the columns d, d + 32, ...
 // final_row: the output row, divided by l; else part_row gets the sums.
@@ -850,15 +834,23 @@ int64_t tile_count(const SeqProblem& p) {
   return most < p.tokens_q ? (most > 0 ? most : 1) : p.tokens_q;
 }
 
-// Blocks that share a tile's keys: as many as one wave of the SMs holds, each
-// with at least four key blocks if the longest sequence is as long as it can
-// be.
+// Blocks that share a tile's keys.  With fewer tiles than a few waves of the
+// SMs hold, the longest ones end long after the others: the split that
+// minimises waves x (key blocks a thread block walks + what its beginning, end
+// and partial result cost, about as long as kSplitCost key blocks take), if it
+// promises a fifth.  Lengths are on the device; the estimate takes the longest
+// they can be.
+constexpr int kSplitCost = 5;
 int tile_splits(const SeqProblem& p, const DeviceInfo& dev) {
-  const int64_t blocks = tile_count(p) * p.heads_kv;
-  const int64_t keys = ((p.table != nullptr ? p.max_keys : p.tokens_kv) + 127) / 128;
-  int64_t n = dev.num_sms / blocks;
-  if (n > (keys + 3) / 4) n = (keys + 3) / 4;
-  return n < 1 ? 1 : int(n);
+  const int64_t blocks = tile_count(p) * p.heads_kv, sms = dev.num_sms;
+  const int64_t keys = (int64_t(p.table != nullptr ? p.max_keys : p.tokens_kv) + 127) / 128;
+  if (blocks >= 4 * sms) return 1;
+  const auto cost = [&](int64_t n) { return (blocks * n + sms - 1) / sms * ((keys + n - 1) / n + kSplitCost); };
+  int64_t best = 1;
+  const int64_t most = keys < 2 * sms ? (keys + 1) / 2 : sms;
+  for (int64_t n = 2; n <= most && blocks * n <= 4 * sms; ++n)
+    if (cost(n) < cost(best)) best = n;
+  return cost(best) * 5 < cost(1) * 4 ? int(best) : 1;
 }
 
 }  // namespace

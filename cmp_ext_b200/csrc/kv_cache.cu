@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 
 #include <climits>
+#include <cstring>
 #include <type_traits>
 
 #include "attention_math.cuh"
@@ -30,15 +31,36 @@ struct CacheCall {
   Side side[2];
   const int64_t* slots;
   int64_t slot_end;  // pages * page_size
-  int64_t vectors;   // tokens * heads
+  uint32_t vectors;  // tokens * heads (32 bits: a 64-bit division for each lane took longer than its memory traffic)
   int heads, d, page_size;
 };
 
-// N consecutive values of a vector as one access.
+// N consecutive values of a vector, moved as one access of their whole size
+// (copied as a struct of bytes they would be loaded one by one).
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Pack {
   T v[N];
 };
+template <int BYTES>
+struct Raw;
+template <> struct Raw<1> { using type = uint8_t; };
+template <> struct Raw<2> { using type = uint16_t; };
+template <> struct Raw<4> { using type = uint32_t; };
+template <> struct Raw<8> { using type = uint2; };
+template <> struct Raw<16> { using type = uint4; };
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  const auto r = *reinterpret_cast<const typename Raw<sizeof(Pack<T, N>)>::type*>(p);
+  Pack<T, N> x;
+  memcpy(&x, &r, sizeof(x));
+  return x;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) {
+  typename Raw<sizeof(x)>::type r;
+  memcpy(&r, &x, sizeof(x));
+  *reinterpret_cast<decltype(r)*>(p) = r;
+}
 
 // e4m3 scale byte of a vector whose largest magnitude is a: the exponent of
 // the smallest power of two 2^e with a <= 448 * 2^e = 1.75 * 2^(e + 8).  Both
@@ -57,13 +79,29 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// Largest magnitude of a pack, NaN if one is.
+template <typename T, int N>
+__device__ __forceinline__ float top_of(const Pack<T, N>& x) {
+  if constexpr (sizeof(T) == 2 && N >= 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 top = __habs2(*reinterpret_cast<const T2*>(&x.v[0]));
+#pragma unroll
+    for (int k = 2; k < N; k += 2) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const T2*>(&x.v[k])));
+    return max_nan(ldf(reinterpret_cast<const T*>(&top)), ldf(reinterpret_cast<const T*>(&top) + 1));
+  } else {
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) top = max_nan(top, fabsf(ldf(&x.v[k])));
+    return top;
+  }
+}
+
 struct Place {
   int64_t page;
   int row;
   bool there;
 };
-__device__ __forceinline__ Place place_of(const CacheCall& c, int64_t token) {
-  const int64_t slot = __ldg(c.slots + token);
+__device__ __forceinline__ Place place_of(const CacheCall& c, int64_t slot) {
   Place r;
   r.there = slot >= 0 && slot < c.slot_end;
   if (c.slot_end <= INT_MAX) {  // the usual case: a 32-bit division
@@ -80,20 +118,25 @@ __device__ __forceinline__ Place place_of(const CacheCall& c, int64_t token) {
 
 // A group of 2^lg lanes owns one vector of keys and the same token's vector
 // of values; a lane holds NC chunks of VEC consecutive values of each, so the
-// largest magnitude takes lg shuffles and the vector is read once.
-// Bound by memory: a token's row moves once each way.
+// largest magnitude takes lg shuffles and the vector is read once, before the
+// slot that says where it goes is needed.
+//
+// Bound by memory once the instructions are few: 64-bit divisions, one chunk
+// a lane and conversions value by value made 16384 tokens of 8 heads of 128
+// (bf16 to e4m3) take 36 us, with 32-bit ones, two chunks a lane and pairs
+// 23 us (4.4 TB/s); several vectors a lane lose more threads than they hide
+// latency (25 us with two, 59 with four).
 template <typename T, bool Q8, int VEC, int NC>
 __global__ void __launch_bounds__(256) kv_write_kernel(const CacheCall c, int lg) {
   using C = typename std::conditional<Q8, __nv_fp8_storage_t, T>::type;
   pdl_trigger();
   pdl_wait();
-  const int64_t vec = (blockIdx.x * 256LL + threadIdx.x) >> lg;
+  const uint32_t vec = blockIdx.x * (256u >> lg) + (threadIdx.x >> lg);
   const int lane = threadIdx.x & ((1 << lg) - 1);
   if (vec >= c.vectors) return;  // whole groups leave together
-  const int64_t token = vec / c.heads;
-  const int head = int(vec - token * c.heads);
-  const Place at = place_of(c, token);
-  if (!at.there) return;
+  const uint32_t token = vec / uint32_t(c.heads);
+  const int head = int(vec - token * uint32_t(c.heads));
+  const int64_t slot = __ldg(c.slots + token);
   Pack<T, VEC> x[2][NC];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -101,9 +144,11 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const CacheCall c, int lg
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int d = (lane + (i << lg)) * VEC;
-      if (d < c.d) x[s][i] = *reinterpret_cast<const Pack<T, VEC>*>(src + d);
+      if (d < c.d) x[s][i] = load_pack<T, VEC>(src + d);
     }
   }
+  const Place at = place_of(c, slot);
+  if (!at.there) return;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     C* dst = static_cast<C*>(c.side[s].cache) + at.page * c.side[s].c_page + head * c.side[s].c_head +
@@ -112,9 +157,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const CacheCall c, int lg
       float a = 0.0f;
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if ((lane + (i << lg)) * VEC < c.d)
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) a = max_nan(a, fabsf(ldf(&x[s][i].v[k])));
+        if ((lane + (i << lg)) * VEC < c.d) a = max_nan(a, top_of(x[s][i]));
       // the lanes of a group leave the kernel together, so they are the mask
       const unsigned mask = lg == 5 ? 0xffffffffu : ((1u << (1 << lg)) - 1u) << (threadIdx.x & 31 & ~((1 << lg) - 1));
       for (int o = 1 << lg >> 1; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(mask, a, o));
@@ -125,9 +168,18 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const CacheCall c, int lg
         const int d = (lane + (i << lg)) * VEC;
         if (d >= c.d) continue;
         Pack<C, VEC> q;
+        if constexpr (VEC == 1) {
+          q.v[0] = __nv_cvt_float_to_fp8(ldf(&x[s][i].v[0]) * down, __NV_SATFINITE, __NV_E4M3);
+        } else {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) q.v[k] = __nv_cvt_float_to_fp8(ldf(&x[s][i].v[k]) * down, __NV_SATFINITE, __NV_E4M3);
-        *reinterpret_cast<Pack<C, VEC>*>(dst + d) = q;
+          for (int k = 0; k < VEC; k += 2) {
+            const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(
+                make_float2(ldf(&x[s][i].v[k]) * down, ldf(&x[s][i].v[k + 1]) * down), __NV_SATFINITE, __NV_E4M3);
+            q.v[k] = uint8_t(two);
+            q.v[k + 1] = uint8_t(two >> 8);
+          }
+        }
+        store_pack(dst + d, q);
       }
       if (lane == 0)
         c.side[s].scale[at.page * c.side[s].s_page + head * c.side[s].s_head + at.row * c.side[s].s_row] = uint8_t(b);
@@ -135,7 +187,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const CacheCall c, int lg
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const int d = (lane + (i << lg)) * VEC;
-        if (d < c.d) *reinterpret_cast<Pack<T, VEC>*>(dst + d) = x[s][i];
+        if (d < c.d) store_pack(dst + d, x[s][i]);
       }
     }
   }
@@ -151,59 +203,70 @@ __device__ __forceinline__ void st_sat(T* p, float x) {
   stf(p, x > top ? top : x < -top ? -top : x);
 }
 
+// The other way, with the same layout of threads.  The slot's latency and the
+// codes' cannot overlap within a thread: 65500 tokens of 8 heads of 128 (e4m3
+// to bf16, scattered slots) take 87 us (4.7 TB/s), 131 us before the same
+// changes.
 template <typename T, bool Q8, int VEC, int NC>
 __global__ void __launch_bounds__(256) kv_read_kernel(const CacheCall c, int lg) {
   using C = typename std::conditional<Q8, __nv_fp8_storage_t, T>::type;
   pdl_trigger();
   pdl_wait();
-  const int64_t vec = (blockIdx.x * 256LL + threadIdx.x) >> lg;
+  const uint32_t vec = blockIdx.x * (256u >> lg) + (threadIdx.x >> lg);
   const int lane = threadIdx.x & ((1 << lg) - 1);
   if (vec >= c.vectors) return;
-  const int64_t token = vec / c.heads;
-  const int head = int(vec - token * c.heads);
-  const Place at = place_of(c, token);
+  const uint32_t token = vec / uint32_t(c.heads);
+  const int head = int(vec - token * uint32_t(c.heads));
+  const Place at = place_of(c, __ldg(c.slots + token));
   Pack<C, VEC> x[2][NC];
-  float up[2];
+  uint8_t scale[2] = {0, 0};
+  if (at.there) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const C* src = static_cast<const C*>(c.side[s].cache) + at.page * c.side[s].c_page + head * c.side[s].c_head +
-                   at.row * c.side[s].c_row;
-    if (Q8 && at.there)
-      up[s] = e8m0_to_float(c.side[s].scale[at.page * c.side[s].s_page + head * c.side[s].s_head + at.row * c.side[s].s_row]);
+    for (int s = 0; s < 2; ++s) {
+      const C* src = static_cast<const C*>(c.side[s].cache) + at.page * c.side[s].c_page + head * c.side[s].c_head +
+                     at.row * c.side[s].c_row;
+      if (Q8) scale[s] = c.side[s].scale[at.page * c.side[s].s_page + head * c.side[s].s_head + at.row * c.side[s].s_row];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int d = (lane + (i << lg)) * VEC;
-      if (at.there && d < c.d) x[s][i] = *reinterpret_cast<const Pack<C, VEC>*>(src + d);
+      for (int i = 0; i < NC; ++i) {
+        const int d = (lane + (i << lg)) * VEC;
+        if (d < c.d) x[s][i] = load_pack<C, VEC>(src + d);
+      }
     }
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     T* dst = static_cast<T*>(c.side[s].x) + token * c.side[s].x_token + head * c.side[s].x_head;
+    const float up = e8m0_to_float(scale[s]);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int d = (lane + (i << lg)) * VEC;
       if (d >= c.d) continue;
       Pack<T, VEC> y;
+      if (!at.there) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        if constexpr (Q8) {
-          const float f = __half2float(__half(__nv_cvt_fp8_to_halfraw(x[s][i].v[k], __NV_E4M3)));
-          st_sat(&y.v[k], at.there ? f * up[s] : 0.0f);
-        } else {
-          if (at.there) y.v[k] = x[s][i].v[k];
-          else stf(&y.v[k], 0.0f);
+        for (int k = 0; k < VEC; ++k) stf(&y.v[k], 0.0f);
+      } else if constexpr (!Q8) {
+        y = x[s][i];
+      } else if constexpr (sizeof(T) == 2 && VEC >= 2) {
+#pragma unroll
+        for (int k = 0; k < VEC; k += 2) {
+          const uint32_t two = dequant2(uint32_t(x[s][i].v[k]) | uint32_t(x[s][i].v[k + 1]) << 8, up, (T*)nullptr);
+          memcpy(&y.v[k], &two, 4);
         }
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          st_sat(&y.v[k], __half2float(__half(__nv_cvt_fp8_to_halfraw(x[s][i].v[k], __NV_E4M3))) * up);
       }
-      *reinterpret_cast<Pack<T, VEC>*>(dst + d) = y;
+      store_pack(dst + d, y);
     }
   }
 }
 
 template <typename T, bool Q8, int VEC, int NC>
 cudaError_t launch_rows(const CacheCall& c, int lg, bool write, cudaStream_t s) {
-  const int64_t blocks = ((c.vectors << lg) + 255) / 256;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.gridDim = dim3(unsigned(((int64_t(c.vectors) << lg) + 255) / 256));
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -211,7 +274,9 @@ cudaError_t launch_rows(const CacheCall& c, int lg, bool write, cudaStream_t s) 
   return cudaLaunchKernelEx(&cfg, write ? kv_write_kernel<T, Q8, VEC, NC> : kv_read_kernel<T, Q8, VEC, NC>, c, lg);
 }
 
-// wide: 16-byte accesses of T (VEC = 16 / sizeof(T)); otherwise single values.
+// wide: 16-byte accesses of T (VEC = 16 / sizeof(T)), two a lane where the
+// vector has them (a lane's address arithmetic costs as much as its data);
+// otherwise single values.
 template <typename T, bool Q8>
 cudaError_t launch_typed(const CacheCall& c, bool wide, bool write, cudaStream_t s) {
   constexpr int W = 16 / int(sizeof(T));
@@ -220,9 +285,8 @@ cudaError_t launch_typed(const CacheCall& c, bool wide, bool write, cudaStream_t
     while (lg < 5 && (1 << lg) < c.d) ++lg;
     return launch_rows<T, Q8, 1, kSimtMaxD / 32>(c, lg, write, s);
   }
-  while (lg < 5 && (W << lg) < c.d) ++lg;
-  const int chunks = (c.d + (W << lg) - 1) / (W << lg);
-  if (chunks <= 1) return launch_rows<T, Q8, W, 1>(c, lg, write, s);
+  while (lg < 5 && (2 * W << lg) < c.d) ++lg;
+  if (c.d <= (2 * W << lg)) return launch_rows<T, Q8, W, 2>(c, lg, write, s);
   return launch_rows<T, Q8, W, kSimtMaxD / (32 * W)>(c, lg, write, s);
 }
 
@@ -245,7 +309,7 @@ int run_cache(const cmpx_kv_cache_args* a, bool write, cudaStream_t s) {
   if (!empty_cache && q8 && (a->key_scale == nullptr || a->value_scale == nullptr)) return CMPX_ERR_INVALID_ARG;
   if (a->head_dim > kSimtMaxD) return CMPX_ERR_UNSUPPORTED;
   if (a->page_size > INT_MAX || a->heads > INT_MAX || a->tokens > INT_MAX ||
-      a->tokens * a->heads > (int64_t(INT_MAX) * 256 >> 5))
+      a->tokens * a->heads > INT_MAX)
     return CMPX_ERR_UNSUPPORTED;
   if (!empty_cache && a->pages > INT64_MAX / a->page_size) return CMPX_ERR_UNSUPPORTED;
   if (empty_cache && write) return CMPX_OK;  // every slot is outside
@@ -263,7 +327,7 @@ int run_cache(const cmpx_kv_cache_args* a, bool write, cudaStream_t s) {
                    a->vs_stride_head, a->vs_stride_row};
   c.slots = a->slots;
   c.slot_end = empty_cache ? 0 : a->pages * a->page_size;
-  c.vectors = a->tokens * a->heads;
+  c.vectors = uint32_t(a->tokens * a->heads);
   c.heads = int(a->heads);
   c.d = int(a->head_dim);
   c.page_size = empty_cache ? 1 : int(a->page_size);
