@@ -98,16 +98,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Four e4m3 codes as two fp16 pairs (exact): codes 0 and 1, codes 2 and 3.
-__device__ __forceinline__ void e4m3_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(codes));
-}
-__device__ __forceinline__ uint32_t half2_to_bf16(uint32_t h2) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-  return pack2(f.x, f.y, (__nv_bfloat16*)nullptr);
-}
 // An 8 x 8 matrix of 16-bit values, turned.
 __device__ __forceinline__ uint32_t turn8x8(uint32_t a) {
   uint32_t d;

@@ -97,4 +97,43 @@ __device__ __forceinline__ uint32_t dequant2(uint32_t codes, float up, __nv_bflo
   return r;
 }
 
+// Four e4m3 codes as two fp16 pairs (exact): codes 0 and 1, codes 2 and 3.
+__device__ __forceinline__ void e4m3_to_half(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
+}
+__device__ __forceinline__ uint32_t half2_to_bf16(uint32_t h2) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+  return pack2(f.x, f.y, (__nv_bfloat16*)nullptr);
+}
+
+// Whether the scale byte is one that scale4 takes: 2^e such that no code times
+// it leaves T's finite range, and 2^e itself is a normal T.
+__device__ __forceinline__ bool scale4_takes(uint32_t byte, __half*) { return byte >= 113 && byte <= 134; }
+__device__ __forceinline__ bool scale4_takes(uint32_t byte, __nv_bfloat16*) { return byte >= 1 && byte <= 245; }
+// Four e4m3 codes times 2^(byte - 127) in T, as two pairs; rounded like
+// dequant2, with packed multiplications instead of fp32 ones.
+__device__ __forceinline__ void scale4(uint32_t codes, uint32_t byte, uint32_t& lo, uint32_t& hi, __half*) {
+  const uint32_t bits = (byte - 112) << 10, two = bits | bits << 16;
+  uint32_t a, b;
+  e4m3_to_half(codes, a, b);
+  const __half2 s = *reinterpret_cast<const __half2*>(&two);
+  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), s), y = __hmul2(*reinterpret_cast<const __half2*>(&b), s);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ void scale4(uint32_t codes, uint32_t byte, uint32_t& lo, uint32_t& hi, __nv_bfloat16*) {
+  const uint32_t two = byte << 7 | byte << 23;
+  uint32_t a, b;
+  e4m3_to_half(codes, a, b);
+  a = half2_to_bf16(a);
+  b = half2_to_bf16(b);
+  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&two);
+  const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), s),
+                       y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), s);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+
 }  // namespace cmpx

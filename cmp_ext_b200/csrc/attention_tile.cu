@@ -59,11 +59,13 @@ struct TileCfg {
   static constexpr int THREADS = 32 * WARPS;
   static constexpr int QCH = D / 64;            // 128-byte chunks of a 16-bit row
   static constexpr int TILE = 128 * D * 2;      // 128 rows
-  // key and value blocks in flight; 8-bit codes wait in RS raw blocks, keys
-  // and values in turn
-  static constexpr int KS = D == 64 ? 4 : Q8 ? 2 : 3;
+  // key and value blocks in the queries' type; 8-bit codes arrive in RS raw
+  // blocks, keys and values in turn (two of them left the SM waiting for one
+  // load at a time, which took longer than a block's products; a key block is
+  // done with early, so one converted one is enough)
+  static constexpr int KS = D == 64 ? 4 : Q8 ? 1 : 3;
   static constexpr int VS = D == 64 ? 4 : 2;
-  static constexpr int RS = !Q8 ? 0 : D == 64 ? 4 : 2;
+  static constexpr int RS = !Q8 ? 0 : D == 64 ? 8 : 4;
   static constexpr int RAW = 128 * D;
   static constexpr size_t SMEM = size_t(TILE) * (2 + KS + VS) + size_t(RS) * (RAW + 128) + 1024 + 512;
   // registers a thread of the two softmax warpgroups and of the others
@@ -521,26 +523,53 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
         }
         const uint8_t* src = sR + r * Cfg::RAW;
         uint8_t* dst = (isv ? sV : sK) + slot * Cfg::TILE;
+        // four rows' loads before their stores, which the compiler must take
+        // to overlap them (one row at a time: 2400 cycles for a block's keys
+        // or values, more than its products take)
+        constexpr int BATCH = 4;
+#pragma unroll 1
+        for (int k0 = 0; k0 < 128 / RPI; k0 += BATCH) {
+          uint4 codes[BATCH];
+          uint32_t byte[BATCH];
+          bool takes = true;
 #pragma unroll
-        for (int k = 0; k < 128 / RPI; ++k) {
-          const int row = k * RPI + r_in;
-          const uint4 codes = *reinterpret_cast<const uint4*>(src + row * D + c16 * 16);
-          // a row behind the last key may hold anything, NaN too: zeros
-          const bool in = kv0 + row < kend;
-          const float up = in ? e8m0_to_float(sScale[r * 128 + row]) : 0.0f;
-          const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-          uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = in ? w[e] : 0u;
-            h[2 * e] = dequant2(x & 0xffffu, up, (T*)nullptr);
-            h[2 * e + 1] = dequant2(x >> 16, up, (T*)nullptr);
+          for (int b = 0; b < BATCH; ++b) {
+            const int row = (k0 + b) * RPI + r_in;
+            codes[b] = *reinterpret_cast<const uint4*>(src + row * D + c16 * 16);
+            byte[b] = sScale[r * 128 + row];
           }
-          const int unit = (c16 & 3) * 2, flip = c16 >> 2;
-          uint8_t* at = dst + (c16 >> 2) * 16384 + row * 128;
-          const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-          *reinterpret_cast<uint4*>(at + (((unit + flip) ^ (row & 7)) << 4)) = flip ? hi : lo;
-          *reinterpret_cast<uint4*>(at + (((unit + 1 - flip) ^ (row & 7)) << 4)) = flip ? lo : hi;
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            // a row behind the last key may hold anything, NaN too: zeros
+            if (kv0 + (k0 + b) * RPI + r_in >= kend) {
+              codes[b] = make_uint4(0u, 0u, 0u, 0u);
+              byte[b] = 127;
+            }
+            takes = takes && scale4_takes(byte[b], (T*)nullptr);
+          }
+          takes = __all_sync(0xffffffffu, takes);
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            const int row = (k0 + b) * RPI + r_in;
+            const uint32_t w[4] = {codes[b].x, codes[b].y, codes[b].z, codes[b].w};
+            uint32_t h[8];
+            if (takes) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) scale4(w[e], byte[b], h[2 * e], h[2 * e + 1], (T*)nullptr);
+            } else {
+              const float up = e8m0_to_float(byte[b]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                h[2 * e] = dequant2(w[e] & 0xffffu, up, (T*)nullptr);
+                h[2 * e + 1] = dequant2(w[e] >> 16, up, (T*)nullptr);
+              }
+            }
+            const int unit = (c16 & 3) * 2, flip = c16 >> 2;
+            uint8_t* at = dst + (c16 >> 2) * 16384 + row * 128;
+            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+            *reinterpret_cast<uint4*>(at + (((unit + flip) ^ (row & 7)) << 4)) = flip ? hi : lo;
+            *reinterpret_cast<uint4*>(at + (((unit + 1 - flip) ^ (row & 7)) << 4)) = flip ? lo : hi;
+          }
         }
         fence_proxy_async_smem();
         mbar_arrive(isv ? &v_full[slot] : &k_full[slot]);
@@ -557,7 +586,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
     const int token = i0 + t * a.tokens + r / p.group;  // of the sequence
     const int head = hk * p.group + r % p.group;
     const bool valid = seq >= 0 && r < a.tokens * p.group && token < s.n;
-    const int lim = valid ? seq_limit(p, s, token) : 0;
+    // (rows of nothing see all keys, so that they never make a warp mask)
+    const int lim = valid ? seq_limit(p, s, token) : kend;
     const float sl = p.scale_log2;
     float m = -INFINITY, l = 0.0f;  // the reference point of the weights, their sum
     bool ok = true;
@@ -834,23 +864,24 @@ int64_t tile_count(const SeqProblem& p) {
   return most < p.tokens_q ? (most > 0 ? most : 1) : p.tokens_q;
 }
 
-// Blocks that share a tile's keys.  With fewer tiles than a few waves of the
-// SMs hold, the longest ones end long after the others: the split that
-// minimises waves x (key blocks a thread block walks + what its beginning, end
-// and partial result cost, about as long as kSplitCost key blocks take), if it
-// promises a fifth.  Lengths are on the device; the estimate takes the longest
-// they can be.
-constexpr int kSplitCost = 5;
+// Blocks that share a tile's keys.  Two things bound the time, in units of the
+// 2.2 us a key block takes: the longest walk of a block, and all walks over the
+// SMs.  A block's beginning, end and partial result cost as much as five key
+// blocks, the joining kernel two.  Lengths are on the device: the longest walk
+// is taken to be as long as a sequence can be, a typical one 0.6 of it.  (16
+// sequences of 713 new tokens over 200 to 6000 keys: 142 us unsplit, NNMM
+// split in two.)
 int tile_splits(const SeqProblem& p, const DeviceInfo& dev) {
-  const int64_t blocks = tile_count(p) * p.heads_kv, sms = dev.num_sms;
-  const int64_t keys = (int64_t(p.table != nullptr ? p.max_keys : p.tokens_kv) + 127) / 128;
-  if (blocks >= 4 * sms) return 1;
-  const auto cost = [&](int64_t n) { return (blocks * n + sms - 1) / sms * ((keys + n - 1) / n + kSplitCost); };
-  int64_t best = 1;
-  const int64_t most = keys < 2 * sms ? (keys + 1) / 2 : sms;
-  for (int64_t n = 2; n <= most && blocks * n <= 4 * sms; ++n)
+  const double blocks = double(tile_count(p)) * p.heads_kv, sms = dev.num_sms;
+  const double keys = ((p.table != nullptr ? p.max_keys : p.tokens_kv) + 127) / 128;
+  const auto cost = [&](int n) {
+    const double longest = keys / n + 5, all = blocks * (0.6 * keys + 5 * n) / sms;
+    return (longest > all ? longest : all) + (n > 1 ? 2 : 0);
+  };
+  int best = 1;
+  for (int n = 2; n <= dev.num_sms && 2 * n <= keys; ++n)
     if (cost(n) < cost(best)) best = n;
-  return cost(best) * 5 < cost(1) * 4 ? int(best) : 1;
+  return best;
 }
 
 }  // namespace
