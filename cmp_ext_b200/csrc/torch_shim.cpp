@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -455,6 +456,33 @@ void check_writable(const torch::Tensor& t, const char* name, bool unit_last) {
   }
 }
 
+// Whether `delta` elements lie between two places of a tensor with these
+// (stride, size) pairs, largest stride first, none of whose elements share an
+// address.
+bool reaches(const std::vector<std::pair<int64_t, int64_t>>& dims, size_t i, int64_t delta) {
+  if (i == dims.size()) return delta == 0;
+  const int64_t stride = dims[i].first, most = dims[i].second - 1;
+  const int64_t down = delta >= 0 ? delta / stride : -((-delta + stride - 1) / stride);
+  for (int64_t d : {down, down + 1})
+    if (d >= -most && d <= most && reaches(dims, i + 1, delta - d * stride)) return true;
+  return false;
+}
+
+// Two tensors that a kernel writes together (both passed check_writable) share
+// an element.  Views of one buffer may lie between each other's rows if they
+// have the same layout; with different ones their ranges must be apart.
+bool share_elements(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0 || !overlaps(a, b)) return false;
+  if (a.sizes() != b.sizes() || a.strides() != b.strides() || a.element_size() != b.element_size()) return true;
+  const int64_t bytes = static_cast<const char*>(a.data_ptr()) - static_cast<const char*>(b.data_ptr());
+  if (bytes % a.element_size() != 0) return true;
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1) dims.emplace_back(a.stride(i), a.size(i));
+  std::sort(dims.rbegin(), dims.rend());
+  return reaches(dims, 0, bytes / a.element_size());
+}
+
 // query / key / value as the kernels take them: unit stride along D, and for
 // 16-bit types strides and addresses on 16 bytes (a copy otherwise).
 torch::Tensor rows16(torch::Tensor t) {
@@ -481,14 +509,14 @@ torch::Tensor index_arg(const torch::Tensor& t, const char* name, int64_t size, 
 }
 
 torch::Tensor seq_output(const c10::optional<torch::Tensor>& out, const torch::Tensor& query,
-                         const std::vector<torch::Tensor>& inputs) {
+                         std::initializer_list<const torch::Tensor*> inputs) {
   if (!out.has_value() || !out->defined()) return torch::empty(query.sizes(), query.options());
   TORCH_CHECK(out->sizes() == query.sizes(), "out must have the query's shape");
   TORCH_CHECK(out->scalar_type() == query.scalar_type(), "out must have the query's dtype");
   TORCH_CHECK(out->device() == query.device(), "Device mismatch");
   check_writable(*out, "out", true);
-  for (const auto& t : inputs)
-    if (t.defined()) TORCH_CHECK(!overlaps(*out, t), "out must not overlap an input");
+  for (const torch::Tensor* t : inputs)
+    if (t != nullptr && t->defined()) TORCH_CHECK(!overlaps(*out, *t), "out must not overlap an input");
   return *out;
 }
 
@@ -550,7 +578,7 @@ torch::Tensor attention_varlen(torch::Tensor query, torch::Tensor key, torch::Te
     TORCH_CHECK(key.size(0) == query.size(0), "Without cu_seqlens_k, key must have as many tokens as query");
   TORCH_CHECK(query.is_cuda(), "attention_varlen expects CUDA tensors");
   c10::cuda::CUDAGuard guard(query.device());
-  torch::Tensor out = seq_output(out_arg, query, {query, key, value, cu_seqlens_q, cu_k});
+  torch::Tensor out = seq_output(out_arg, query, {&query, &key, &value, &cu_seqlens_q, &cu_k});
   query = rows16(query);
   key = rows16(key);
   value = rows16(value);
@@ -641,9 +669,8 @@ torch::Tensor attention_paged(torch::Tensor query, torch::Tensor key_cache, torc
   TORCH_CHECK(query.is_cuda(), "attention_paged expects CUDA tensors");
   c10::cuda::CUDAGuard guard(query.device());
   torch::Tensor out = seq_output(out_arg, query,
-                                 {query, key_cache, value_cache, page_table, seqlens_k, cu_q,
-                                  kv == CMPX_E4M3 ? *key_scale : torch::Tensor(),
-                                  kv == CMPX_E4M3 ? *value_scale : torch::Tensor()});
+                                 {&query, &key_cache, &value_cache, &page_table, &seqlens_k, &cu_q,
+                                  kv == CMPX_E4M3 ? &*key_scale : nullptr, kv == CMPX_E4M3 ? &*value_scale : nullptr});
   query = rows16(query);
   lens = lens.contiguous();
   if (cu_q.defined()) cu_q = cu_q.contiguous();
@@ -745,8 +772,10 @@ void kv_cache_write(torch::Tensor key, torch::Tensor value, torch::Tensor key_ca
   for (size_t i = 0; i < written.size(); ++i) {
     check_writable(written[i].first, written[i].second, i < 2);
     for (size_t j = 0; j < i; ++j)
-      TORCH_CHECK(written[i].first.numel() == 0 || written[i].first.data_ptr() != written[j].first.data_ptr(),
-                  written[i].second, " must not be ", written[j].second);
+      TORCH_CHECK(!share_elements(written[i].first, written[j].first), written[i].second, " must not be ",
+                  written[j].second, " or overlap it");
+    for (const torch::Tensor* t : {&key, &value, &slots})
+      TORCH_CHECK(!overlaps(written[i].first, *t), written[i].second, " must not overlap an input");
   }
   TORCH_CHECK(key.is_cuda(), "kv_cache_write expects CUDA tensors");
   c10::cuda::CUDAGuard guard(key.device());

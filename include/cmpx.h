@@ -244,8 +244,13 @@ CMPX_API int cmpx_attention_select_path(int dtype, const void* Q, const void* K,
  * Softmax statistics and sums are fp32; the output is rounded once.  fp16 /
  * bf16 with head_dim 64 or 128 run tensor-core kernels (a flash-decoding
  * kernel for few query rows per kv head, a tcgen05 kernel for more; softmax
- * weights are rounded to 16 bits once); fp32 and other head_dim up to 512, or
- * layouts TMA cannot describe, run a CUDA-core kernel.
+ * weights are rounded to 16 bits once, to bf16's where the scales of an 8-bit
+ * cache's values differ by more than 2^6 up or 2^10 down from a block's first
+ * ones).  They take pages of 8, 16, 32, ... keys (8-bit caches: 16, 32, ...,
+ * with contiguous scales of a page), 16-byte aligned addresses and strides of
+ * 16-byte multiples.  fp32, other head_dim up to 512 and other layouts run a
+ * CUDA-core kernel, which is correct but slow.  Values of an 8-bit cache are
+ * taken in the queries' type, held to its finite range.
  *
  * All strides are in elements.  The element stride within a head is 1. */
 typedef struct {
@@ -274,7 +279,7 @@ typedef struct {
   float scale;
   int causal;
   int zero_rest;        /* 1: rows of O outside every sequence are zeroed; 0: they are left as they were */
-  int64_t max_seqlen_q; /* longest sequence's new tokens if known (picks the kernel, never the result); 0: unknown */
+  int64_t max_seqlen_q; /* longest sequence's new tokens if known (only picks the kernel); 0: unknown */
   int path;             /* CMPX_PATH_AUTO, CMPX_PATH_TC (tcgen05), CMPX_PATH_SKINNY (flash decoding), CMPX_PATH_SIMT */
   void* workspace;      /* device, 16-byte aligned, cmpx_attention_seq_workspace_size() bytes (NULL if that is 0);
                            contents need no preparation and do not survive the call */

@@ -111,6 +111,23 @@ def test_cache_checks():
     raises("expects CUDA tensors", r, kc, vc, slots)
 
 
+def test_cache_overlaps_are_refused():
+    w = cx.kv_cache_write
+    k = torch.zeros(5, 2, 8)
+    slots = torch.zeros(5, dtype=torch.int64)
+    buf = torch.zeros(8, 2, 4, 8)
+    raises("value_cache must not be key_cache or overlap it", w, k, k, buf[:6], buf[2:], slots)
+    raises("value_cache must not be key_cache or overlap it", w, k, k, buf[:4], buf.view(-1)[8:8 + 256].view(4, 2, 4, 8), slots)
+    raises("key_cache must not overlap an input", w, buf.view(-1)[:80].view(5, 2, 8), k, buf, torch.zeros_like(buf), slots)
+    # both in one buffer, page by page or side by side: shared by nobody, so the next check is reached
+    pair = torch.zeros(3, 2, 2, 4, 8)
+    raises("expects CUDA tensors", w, k, k, pair[:, 0], pair[:, 1], slots)
+    wide = torch.zeros(3, 2, 4, 16)
+    raises("expects CUDA tensors", w, k, k, wide[..., :8], wide[..., 8:], slots)
+    raises("value_cache must not be key_cache or overlap it", w, k, k, wide[..., :8], wide[..., 7:15], slots)
+    raises("expects CUDA tensors", w, k, k, buf[:4], buf[4:], slots)
+
+
 # ---------------------------------------------------------------- C ABI
 def seq_args(**kw):
     a = cabi.AttentionSeqArgs()
@@ -164,6 +181,37 @@ def test_seq_empty_and_too_large():
     assert run(seq_args(head_dim=513)) == cabi.ERR_UNSUPPORTED
     assert run(seq_args(tokens_q=2**31)) == cabi.ERR_UNSUPPORTED
     assert run(paged_args(max_pages=2**31)) == cabi.ERR_UNSUPPORTED
+
+
+def select(a):
+    return cabi.lib().cmpx_attention_seq_select_path(ctypes.byref(a))
+
+
+def test_path_selection_is_host_logic():
+    assert select(seq_args()) == cabi.PATH_SKINNY                       # 4 tokens a sequence x 2 heads
+    assert select(seq_args(tokens_q=64, tokens_kv=64)) == cabi.PATH_TC   # 32 tokens
+    assert select(seq_args(tokens_q=64, tokens_kv=64, max_seqlen_q=8)) == cabi.PATH_SKINNY
+    assert select(seq_args(max_seqlen_q=9)) == cabi.PATH_TC
+    assert select(seq_args(dtype=cabi.F32, kv_dtype=cabi.F32)) == cabi.PATH_SIMT
+    assert select(seq_args(head_dim=96)) == cabi.PATH_SIMT
+    assert select(seq_args(head_dim=1024)) == -1
+    assert select(seq_args(K=0x200008)) == cabi.PATH_SIMT               # not on 16 bytes
+    assert select(seq_args(k_stride_row=260)) == cabi.PATH_SIMT          # rows not on 16 bytes
+    assert select(seq_args(tokens_kv=0)) == cabi.PATH_SIMT               # no key at all
+    assert select(seq_args(scale=0.0, tokens_q=64)) == cabi.PATH_SKINNY  # the tcgen05 kernel masks with -inf
+    assert select(seq_args(path=cabi.PATH_SIMT)) == cabi.PATH_SIMT
+    assert select(seq_args(path=cabi.PATH_TC, head_dim=96)) == -1
+    wide = dict(heads_q=400, tokens_q=2, k_stride_row=256)
+    assert select(seq_args(**wide)) == cabi.PATH_SKINNY                  # 200 heads a kv head fill no 128-row tile
+    for page, want in ((1, cabi.PATH_SIMT), (4, cabi.PATH_SIMT), (8, cabi.PATH_SKINNY), (24, cabi.PATH_SIMT),
+                       (64, cabi.PATH_SKINNY)):
+        assert select(paged_args(page_size=page)) == want, page
+    e4m3 = dict(kv_dtype=cabi.E4M3, k_scale=0x800000, v_scale=0x900000, ks_stride_row=1, vs_stride_row=1,
+                ks_stride_head=16, vs_stride_head=16, ks_stride_page=32, vs_stride_page=32)
+    assert select(paged_args(**e4m3)) == cabi.PATH_SKINNY
+    assert select(paged_args(**{**e4m3, "ks_stride_row": 2})) == cabi.PATH_SIMT
+    assert select(paged_args(**{**e4m3, "page_size": 8})) == cabi.PATH_SIMT
+    assert select(paged_args(**{**e4m3, "k_stride_row": 136})) == cabi.PATH_SIMT
 
 
 def cache_args(**kw):
