@@ -205,7 +205,7 @@ __device__ __forceinline__ void st_sat(T* p, float x) {
 
 // The other way, with the same layout of threads.  The slot's latency and the
 // codes' cannot overlap within a thread: 65500 tokens of 8 heads of 128 (e4m3
-// to bf16, scattered slots) take 87 us (4.7 TB/s), 131 us before the same
+// to bf16, scattered slots) take 87-94 us (4.3-4.7 TB/s), 131 us before the same
 // changes.
 template <typename T, bool Q8, int VEC, int NC>
 __global__ void __launch_bounds__(256) kv_read_kernel(const CacheCall c, int lg) {
