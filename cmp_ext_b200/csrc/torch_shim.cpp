@@ -435,17 +435,17 @@ std::pair<const char*, const char*> span_of(const torch::Tensor& t) {
   for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
   return {p, p + (last + 1) * t.element_size()};
 }
-bool overlaps(const torch::Tensor& a, const torch::Tensor& b) {
-  const auto x = span_of(a), y = span_of(b);
-  return x.first < y.second && y.first < x.second;
+bool overlaps(const std::pair<const char*, const char*>& x, const std::pair<const char*, const char*>& y) {
+  return x.first < x.second && y.first < y.second && x.first < y.second && y.first < x.second;
 }
+bool overlaps(const torch::Tensor& a, const torch::Tensor& b) { return overlaps(span_of(a), span_of(b)); }
 
 // A tensor that a kernel writes in place: unit stride along D, and no two
 // elements on one address.
 void check_writable(const torch::Tensor& t, const char* name, bool unit_last) {
   if (t.numel() == 0) return;
   TORCH_CHECK(!unit_last || t.stride(-1) == 1 || t.size(-1) == 1, name, " must be contiguous along its last dimension");
-  std::vector<std::pair<int64_t, int64_t>> dims;
+  c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;
   for (int64_t i = 0; i < t.dim(); ++i)
     if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
   std::sort(dims.begin(), dims.end());
@@ -764,18 +764,24 @@ void kv_cache_write(torch::Tensor key, torch::Tensor value, torch::Tensor key_ca
   TORCH_CHECK(kv == dt || kv == CMPX_E4M3, "Dtype mismatch");
   check_slots(slots, key);
   TORCH_CHECK(slots.size(0) == key.size(0), "slots must have one element for each token");
-  std::vector<std::pair<torch::Tensor, const char*>> written = {{key_cache, "key_cache"}, {value_cache, "value_cache"}};
+  struct Written {
+    const torch::Tensor* t;
+    const char* name;
+    std::pair<const char*, const char*> span;
+  } written[4] = {{&key_cache, "key_cache", {}}, {&value_cache, "value_cache", {}}};
   if (kv == CMPX_E4M3) {
-    written.emplace_back(*key_scale, "key_scale");
-    written.emplace_back(*value_scale, "value_scale");
+    written[2] = {&*key_scale, "key_scale", {}};
+    written[3] = {&*value_scale, "value_scale", {}};
   }
-  for (size_t i = 0; i < written.size(); ++i) {
-    check_writable(written[i].first, written[i].second, i < 2);
-    for (size_t j = 0; j < i; ++j)
-      TORCH_CHECK(!share_elements(written[i].first, written[j].first), written[i].second, " must not be ",
-                  written[j].second, " or overlap it");
-    for (const torch::Tensor* t : {&key, &value, &slots})
-      TORCH_CHECK(!overlaps(written[i].first, *t), written[i].second, " must not overlap an input");
+  const std::pair<const char*, const char*> inputs[3] = {span_of(key), span_of(value), span_of(slots)};
+  for (int i = 0; i < (kv == CMPX_E4M3 ? 4 : 2); ++i) {
+    Written& w = written[i];
+    check_writable(*w.t, w.name, i < 2);
+    w.span = span_of(*w.t);
+    for (int j = 0; j < i; ++j)
+      TORCH_CHECK(!overlaps(w.span, written[j].span) || !share_elements(*w.t, *written[j].t), w.name, " must not be ",
+                  written[j].name, " or overlap it");
+    for (const auto& in : inputs) TORCH_CHECK(!overlaps(w.span, in), w.name, " must not overlap an input");
   }
   TORCH_CHECK(key.is_cuda(), "kv_cache_write expects CUDA tensors");
   c10::cuda::CUDAGuard guard(key.device());
