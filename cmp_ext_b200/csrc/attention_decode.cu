@@ -16,10 +16,11 @@
 // head of the group) along the 8-wide one.  Eight rows waste half of what
 // sixteen would, and a warp's state (D x 8 sums) leaves registers for sixteen
 // warps an SM, which is what hides the latency of the strip's chain of
-// dependent steps (with rows along the 16-wide side, twice the products and
-// eight warps, an e4m3 tile took 5200 cycles; now 1400).
+// dependent steps.  48 single tokens of 32 / 8 heads of 128 over 1000 to 24000
+// keys in an e4m3 cache: 440 us with rows along the 16-wide side, 122 us now
+// (5.7 TB/s of what it has to read, 88% of the copy rate).
 //
-// Work: units (sequence, kv head, ROWS rows) of ceil(keys / 64) tiles in one
+// Work: units (sequence, kv head, ROWS rows) of tiles (64 or 128 keys) in one
 // list, each unit's beginning and end weighted like two tiles; block c of P
 // takes the places [c W / P, (c + 1) W / P) of W, so ragged lengths and few
 // sequences load every SM alike, and its loads run ahead across unit borders.
@@ -45,7 +46,8 @@
 // of it; a strip with another one takes bf16 weights, whose range is fp32's.
 //
 // Values that are not finite: as in attention_tile.cu, a row whose result is
-// not finite although its sum is is computed again over its visible keys.
+// not finite although its sum is, and that may not see one of them, is
+// computed again over its visible keys.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -89,14 +91,14 @@ template <bool BF>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (BF)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // An 8 x 8 matrix of 16-bit values, turned.
 __device__ __forceinline__ uint32_t turn8x8(uint32_t a) {
@@ -870,7 +872,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
           if (!a.whole && (flags & kFirst) && lane == 0)
             a.joints[int64_t(info.q0 + row.token) * p.heads_q + row.head] =
                 int(blockIdx.x) | info.pieces << 12 | r << 24;
-          if (__any_sync(0xffffffffu, bad) && tot[y].y > 0.0f && tot[y].y <= 3.4028234663852886e38f) {
+          if (__any_sync(0xffffffffu, bad) && tot[y].y > 0.0f && tot[y].y <= 3.4028234663852886e38f &&
+              seq_hidden_bad<typename std::conditional<Q8, uint8_t, T>::type, D>(
+                  p, info.b, info.k0, info.hk, max(row.lim, info.piece_key), min(info.len, info.key + KEYS))) {
             const T* q = static_cast<const T*>(p.Q) + int64_t(info.q0 + row.token) * p.q_token + row.head * p.q_head;
             redo_row<T, D, Q8>(p, info.b, info.k0, info.hk, q, info.piece_key, min(row.lim, info.key + KEYS), tot[y].x,
                                acc[y]);

@@ -72,6 +72,35 @@ __device__ __forceinline__ void rec_err(int* err, volatile int* abort, int code)
   *abort = 1;
   atomicCAS(err, 0, code);
 }
+// Whether a value of keys [from, to) of a sequence is not finite (a warp
+// looks; T the values' type, or uint8_t for e4m3 codes).  A row whose result
+// is not finite although its sum is has to be computed again only if such a
+// value is among those it may not see: it reaches the row through 0 * NaN.
+template <typename T, int D>
+__device__ __forceinline__ bool seq_hidden_bad(const SeqProblem& p, int b, int k0, int hk, int from, int to) {
+  const int lane = threadIdx.x & 31;
+  bool bad = false;
+  for (int j = from; j < to; ++j) {
+    int64_t at = int64_t(k0 + j) * p.v.row;
+    if (p.table != nullptr) {
+      const int page = __ldg(p.table + b * p.table_stride + j / p.page_size), slot = j % p.page_size;
+      if (page < 0 || page >= p.pages) continue;  // zeros
+      at = page * p.v.page + slot * p.v.row;
+      if (sizeof(T) == 1) bad = bad || p.v.scale[page * p.v.s_page + hk * p.v.s_head + slot * p.v.s_row] == 255;
+    }
+    const T* v = static_cast<const T*>(p.v.base) + at + hk * p.v.head;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      if constexpr (sizeof(T) == 1) {
+        bad = bad || (v[lane + 32 * i] & 0x7f) == 0x7f;
+      } else {
+        const float x = float(v[lane + 32 * i]);
+        bad = bad || x - x != 0.0f;
+      }
+    }
+  }
+  return __any_sync(0xffffffffu, bad);
+}
 // First token that no sequence holds any more (cu_seqlens_q[batch], clamped),
 // and the number of tokens before the first sequence.
 __device__ __forceinline__ int2 seq_rest(const SeqProblem& p) {

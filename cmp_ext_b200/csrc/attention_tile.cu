@@ -14,7 +14,11 @@
 // Per key block and tile the tensor core computes S = Q K^T (512 cycles at
 // D = 128) and O += P V (512), and 128 threads, one a row, turn S into P:
 // 16384 exponentials at 16 a cycle are 1024 cycles.  Two tiles in turn keep
-// both units busy.  S is read into registers and P written over it in tensor
+// both units busy.  Measured: 4300 cycles a key block of both tiles (2048
+// would be the units' own time), 577 us and 920 TFLOP/s on two prompts of 8192
+// tokens, 16 / 4 heads of 128, at clocks that the power limit holds near
+// 1.6 GHz; what is left is each tile's chain of softmax (1800 cycles), P V,
+// its completion and the next Q K^T (1500).  S is read into registers and P written over it in tensor
 // memory, from where the P V product takes it as its A operand: P crosses
 // neither shared memory, whose bandwidth the two products' operands need
 // (the same product from shared memory would read 64 KB a block and tile
@@ -36,8 +40,9 @@
 //
 // Values that are not finite and that some rows of a tile see and others do
 // not (a causal edge) still reach every row through 0 * NaN.  Finite inputs
-// never pay for that: a row whose result is not finite although its sum is is
-// computed again from its definition, one warp a row.
+// never pay for that: a row whose result is not finite although its sum is,
+// and that has such a value among the keys it may not see, is computed again
+// from its definition, one warp a row.
 //
 // Few tiles: the key blocks of a tile are split among gridDim.z thread
 // blocks, which write unnormalised sums, maxima and fp32 accumulators to the
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
       // A tile's P V and next Q K^T go out together, so that the two tiles
       // fall out of step: one is in softmax while the other's products run
       // (issued as they became ready, both tiles' softmax ran at once and the
-      // tensor core waited: 5500 cycles a block of both, now NNNN).
+      // tensor core waited: 5500 cycles a block of both, now 4300).
       uint32_t idle = 0;  // polls since the last product
       uint64_t t0 = 0;
       while (ok && (pv[0] < n0 || pv[1] < n1)) {
@@ -732,6 +737,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
         again &= again - 1;
         const int tok = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
         const int kl = min(__shfl_sync(0xffffffffu, lim, src), kend);
+        if (!seq_hidden_bad<typename std::conditional<Q8, uint8_t, T>::type, D>(p, seq, s.k0, hk, max(kl, jb * 128),
+                                                                               min(kend, (jb + nt) * 128)))
+          continue;
         const float mm = __shfl_sync(0xffffffffu, m, src), ii = __shfl_sync(0xffffffffu, inv, src);
         const T* q = static_cast<const T*>(p.Q) + (s.q0 + tok) * p.q_token + hd * p.q_head;
         T* of = static_cast<T*>(p.O) + (s.q0 + tok) * p.o_token + hd * p.o_head;
@@ -869,7 +877,7 @@ int64_t tile_count(const SeqProblem& p) {
 // SMs.  A block's beginning, end and partial result cost as much as five key
 // blocks, the joining kernel two.  Lengths are on the device: the longest walk
 // is taken to be as long as a sequence can be, a typical one 0.6 of it.  (16
-// sequences of 713 new tokens over 200 to 6000 keys: 142 us unsplit, NNMM
+// sequences of 713 new tokens over 200 to 6000 keys: 142 us unsplit, 110
 // split in two.)
 int tile_splits(const SeqProblem& p, const DeviceInfo& dev) {
   const double blocks = double(tile_count(p)) * p.heads_kv, sms = dev.num_sms;

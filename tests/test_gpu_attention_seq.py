@@ -442,6 +442,62 @@ def test_paged_beyond_32_bit_offsets(cuda):
     assert torch.equal(k2, v) and torch.equal(v2, k)
 
 
+@pytest.mark.parametrize("n", [1, 6, 40])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_paged_bad_tokens_of_an_8_bit_cache(cuda, n, dtype, bad):
+    """A token whose key or value held a NaN or an infinity reads back as NaN:
+    rows that see it are NaN in that kv head, the others keep the bound."""
+    length, at, hkv = 210, 205, 2
+    c = Paged([length], 16, hkv, 64, dtype, "e4m3", seed=14, rest=0.0)
+    q = queries(n, 4, 64, dtype)
+    slot = c.table[0, at // 16].long() * 16 + at % 16
+    k, v = (torch.randn(1, hkv, 64, generator=gen(15), device="cuda").to(dtype) for _ in range(2))
+    for side in range(2):
+        kk, vv = k.clone(), v.clone()
+        (kk, vv)[side][0, 1, 7] = bad
+        cx.kv_cache_write(kk, vv, c.kc, c.vc, slot.view(1), c.ks, c.vs)
+        for x, held in ((kk, c.keys), (vv, c.values)):
+            code, byte = quantise(x)
+            held[0][at] = (code * e8m0(byte).unsqueeze(-1))[0]
+        out = c.run(q)
+        finish()
+        sees = torch.arange(n, device="cuda") + length - n >= at
+        assert out[sees][:, 2:].isnan().all() and out[sees][:, :2].isfinite().all()
+        assert out[~sees].isfinite().all()
+        c.check(out, q, cu_of([n]), True, 1 / 8)
+
+
+def test_workspace_errors_of_the_c_abi(cuda):
+    import ctypes
+
+    q = torch.zeros(1, 8, 128, dtype=BF16, device="cuda")
+    kc = torch.zeros(64, 2, 64, 128, dtype=BF16, device="cuda")
+    table, lens = torch.arange(64, dtype=torch.int32, device="cuda"), torch.tensor([4000], dtype=torch.int32, device="cuda")
+    a = cabi.AttentionSeqArgs()
+    a.dtype = a.kv_dtype = cabi.BF16
+    a.Q, a.K, a.V, a.O = q.data_ptr(), kc.data_ptr(), kc.data_ptr(), torch.empty_like(q).data_ptr()
+    a.batch, a.tokens_q, a.heads_q, a.heads_kv, a.head_dim = 1, 1, 8, 2, 128
+    a.q_stride_token = a.o_stride_token = 1024
+    a.q_stride_head = a.o_stride_head = a.k_stride_row = a.v_stride_row = 128
+    a.k_stride_head = a.v_stride_head = 64 * 128
+    a.k_stride_page = a.v_stride_page = 2 * 64 * 128
+    a.page_table, a.seqlens_k, a.max_pages, a.pages, a.page_size = table.data_ptr(), lens.data_ptr(), 64, 64, 64
+    a.page_table_stride, a.scale, a.causal = 64, 0.1, 1
+    need = cabi.lib().cmpx_attention_seq_workspace_size(ctypes.byref(a))
+    assert need > 0
+    call = lambda: cabi.lib().cmpx_attention_seq(ctypes.byref(a), None)  # noqa: E731
+    assert call() == cabi.ERR_INVALID_ARG  # none
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need - 1
+    assert call() == cabi.ERR_WORKSPACE
+    a.workspace_bytes = need
+    assert call() == cabi.OK
+    a.workspace = ws.data_ptr() + 4
+    assert call() == cabi.ERR_INVALID_ARG  # not on 16 bytes
+    finish()
+
+
 # ---------------------------------------------------------------- streams, graphs, threads
 def test_streams_and_concurrent_calls(cuda):
     c = Paged([5000, 4000, 100], 64, 2, 128, BF16, "e4m3", seed=11)
