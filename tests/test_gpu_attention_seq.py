@@ -604,3 +604,53 @@ def test_random_cases(cuda):
             out = cx.attention_varlen(q, k, v, cu, cu_of(lens), causal=causal)
             finish()
             c.check(out, q, cu, causal, 1 / math.sqrt(d), f"trial {trial}, packed")
+
+
+@pytest.mark.parametrize("kv", ["same", "e4m3"])
+@pytest.mark.parametrize("hq,page,longest", [(300, 1024, 3), (4, 64, 1), (4, 64, 60)])
+def test_sequences_that_share_their_pages(cuda, hq, page, longest, kv):
+    """One row of the page table for every sequence (a row stride of 0), 150
+    query heads to a kv head, pages longer than a tile."""
+    c = Paged([1500], page, 2, 64, BF16, kv, seed=hq)
+    lens = [1500, 0, 1, 1023, 1024, 1025, 64]
+    n = [min(longest, 1 + 7 * i) for i in range(len(lens))]
+    c.table = c.table[:1].expand(len(lens), -1)
+    c.lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c.keys, c.values = [c.keys[0][:x] for x in lens], [c.values[0][:x] for x in lens]
+    q, cu = queries(sum(n), hq, 64, BF16), cu_of(n)
+    out = c.run(q, cu_seqlens_q=cu)
+    finish()
+    c.check(out, q, cu, True, 1 / 8)
+
+
+@pytest.mark.parametrize("path", ["tc", "skinny", "simt"])
+def test_many_sequences(cuda, path):
+    """More sequences than a block looks through at once, most of them empty."""
+    rng = random.Random(9)
+    n = [rng.choice((0, 0, 0, 1, 2)) for _ in range(1500)]
+    lens = [0 if rng.random() < 0.3 else rng.randint(0, 40) for _ in n]
+    c = Paged(lens, 16, 1, 64, F16, "same", seed=3)
+    q, cu = queries(sum(n), 2, 64, F16), cu_of(n)
+    with forced(path):
+        out = c.run(q, cu_seqlens_q=cu)
+        finish()
+        c.check(out, q, cu, True, 1 / 8)
+        out = cx.attention_varlen(q, torch.cat(c.keys), torch.cat(c.values), cu, cu_of(lens))
+        finish()
+        c.check(out, q, cu, True, 1 / 8, "packed")
+
+
+@pytest.mark.parametrize("kv", ["same", "e4m3"])
+@pytest.mark.parametrize("n", [1, 40])
+def test_context_of_nan(cuda, n, kv):
+    """Every value NaN: a row that sees one is NaN, a row that sees nothing zeros."""
+    lens = [n + 3000, n, 0]
+    c = Paged(lens, 32, 2, 128, BF16, kv, seed=n)
+    if kv == "same":
+        c.vc.fill_(math.nan)
+    else:
+        c.vs.view(torch.uint8).fill_(255)
+    q = queries(3 * n, 8, 128, BF16)
+    out = c.run(q)
+    finish()
+    assert out[: 2 * n].isnan().all() and not out[2 * n :].any()
