@@ -40,10 +40,16 @@
 //
 // An 8-bit cache runs in fp16, where its codes are exact.  bf16 queries are
 // brought into fp16's range by a power of two a row (exact for magnitudes down
-// to 2^-31 of the row's largest), key scales multiply the scores in fp32,
-// value scales the weights, relative to the first strip's largest scale: fp16
-// weights then keep their bits while a strip's scales lie within 2^-10 .. 2^6
-// of it; a strip with another one takes bf16 weights, whose range is fp32's.
+// to 2^-31 of the row's largest), and key scales multiply the scores in fp32.
+// Value scales 2^e join the exponent of the weights that multiply the codes,
+// 2^(s + e - z), against a reference point z of their own, which a row moves
+// like that of its scores: whatever the scales of the keys it sees, in whatever
+// order, these weights stay below 2^8 and its largest one near 2^2, while the
+// sum of 2^(s - m) keeps its own bits; 2^(z - m) joins the two when a piece
+// ends.  A reference shared by the rows of a warp or taken once would let a
+// later, larger scale overflow.  Where a key's scale lies 2^10 and more below
+// z - m (a vector of zeros, whose scale is 1, among tiny ones puts z that high),
+// fp16 might drop its bits: the strip takes bf16 weights, whose range is fp32's.
 //
 // Values that are not finite: as in attention_tile.cu, a row whose result is
 // not finite although its sum is, and that may not see one of them, is
@@ -545,9 +551,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       uint32_t qf[DT][NB][2];               // Q^T: row g of block nb
       float o[DT][NB][4];                   // O^T: two columns, rows 2t and 2t + 1
       float m[NB][2], l[NB][2], qs[NB][2];  // rows 2t, 2t + 1: reference point, sum (this lane's keys), score factor
+      float z[NB][2];                       // 8-bit: reference point of the weights that multiply the codes
       int lim[NB][2];
       int lim_min;                          // of all rows
-      float v_ref = 0.0f;                   // 8-bit: 1 / the scale that value scales are relative to (0: none yet)
       {
         const TileInfo& info = infos[st];
         lim_min = info.len;
@@ -599,7 +605,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
           for (int e = 0; e < 2; ++e) {
             qs[nb][e] = p.scale_log2 * __shfl_sync(0xffffffffu, up, 4 * (2 * t + e));
             lim[nb][e] = __shfl_sync(0xffffffffu, keys, 4 * (2 * t + e));
-            m[nb][e] = kNone;
+            m[nb][e] = z[nb][e] = kNone;
             l[nb][e] = 0.0f;
           }
         }
@@ -650,15 +656,27 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
             }
           }
           const uint8_t* sc = scales + st * Cfg::SCALES + strip * 16 + g;
-          float ks[2] = {1.0f, 1.0f};
+          float ks[2] = {1.0f, 1.0f}, ve[2] = {0.0f, 0.0f};  // scales of keys, exponents of those of values
           if constexpr (Q8) {
             ks[0] = e8m0_to_float(sc[0]);
             ks[1] = e8m0_to_float(sc[8]);
+            ve[0] = e8m0_exponent(sc[KEYS]);
+            ve[1] = e8m0_exponent(sc[KEYS + 8]);
           }
           // in log2 units; hidden scores -inf
-          float s[NB][4];
+          float s[NB][4], c[NB][4];  // c (8-bit): exponents of the weights that multiply the codes
           bool grew = false;
           const bool cut = kv0 + 16 > lim_min;
+          // (behind s, since a hidden value's scale may be a NaN)
+          auto code_exponents = [&](int nb) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[nb][e] = s[nb][e] - z[nb][e & 1] + ve[e >> 1];
+            if (cut) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]) c[nb][e] = -INFINITY;
+            }
+          };
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -672,6 +690,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                 if (kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]) s[nb][e] = -INFINITY;
             }
             grew = grew || fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kGrow || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kGrow;
+            if constexpr (Q8) {
+              code_exponents(nb);
+              grew = grew || fmaxf(fmaxf(c[nb][0], c[nb][1]), fmaxf(c[nb][2], c[nb][3])) > kGrow;
+            }
           }
           if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -683,20 +705,37 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                 for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                 const bool up = mx > m[nb][e] + kGrow;
                 const float m_new = up ? mx - kBias : m[nb][e];
-                const float alpha = up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
+                float alpha = up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
                 m[nb][e] = m_new;
                 l[nb][e] *= alpha;
+                if constexpr (Q8) {
+                  float high = -INFINITY;  // largest score + exponent (hidden ones, -inf and NaN left out)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h)
+                    if (c[nb][e + 2 * h] > -INFINITY) high = fmaxf(high, s[nb][e + 2 * h] + ve[h]);
+#pragma unroll
+                  for (int x = 4; x < 32; x <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
+                  const float z_new = high > z[nb][e] + kGrow ? high - kBias : z[nb][e];
+                  alpha = z_new != z[nb][e] ? ex2_approx(z[nb][e] - z_new) : 1.0f;
+                  z[nb][e] = z_new;
+                }
 #pragma unroll
                 for (int k = 0; k < DT; ++k) {
                   o[k][nb][e] *= alpha;
                   o[k][nb][e + 2] *= alpha;
                 }
               }
+            if constexpr (Q8) {
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) code_exponents(nb);
+            }
           }
+          bool far = false;  // 8-bit: a visible key's scale lies 2^10 and more below z - m
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
+              if constexpr (Q8) far = far || (ve[e >> 1] <= z[nb][e & 1] - m[nb][e & 1] - 10.0f && c[nb][e] > -INFINITY);
               s[nb][e] = ex2_approx(s[nb][e] - m[nb][e & 1]);
               l[nb][e & 1] += s[nb][e];
             }
@@ -728,27 +767,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
             if (tail < 16) add(std::true_type());
             else add(std::false_type());
           } else {
-            float vs[2];
-            vs[0] = e8m0_to_float(sc[KEYS]);
-            vs[1] = e8m0_to_float(sc[KEYS + 8]);
-            if (v_ref == 0.0f) {
-              float top = fmaxf(g < tail ? vs[0] : 0.0f, g + 8 < tail ? vs[1] : 0.0f);  // drops a NaN
-#pragma unroll
-              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-              v_ref = 1.0f / fminf(fmaxf(top, 0x1p-126f), 0x1p126f);
-            }
-            bool near = true;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              vs[h] = g + 8 * h < tail ? vs[h] * v_ref : 1.0f;
-              near = near && vs[h] >= 0x1p-10f && vs[h] <= 0x1p6f;
-            }
-            near = __all_sync(0xffffffffu, near);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)  // (a hidden key's scale may be a NaN, which is not near)
-                s[nb][e] = !near && s[nb][e] == 0.0f ? 0.0f : s[nb][e] * vs[e >> 1];
+              for (int e = 0; e < 4; ++e) c[nb][e] = ex2_approx(c[nb][e]);
             auto add = [&](auto half_type, auto clear) {
               using P = decltype(half_type);
               constexpr bool kBf = std::is_same<P, __nv_bfloat16>::value;
@@ -756,7 +778,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (P*)nullptr));
+                for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(c[nb][2 * h], c[nb][2 * h + 1], (P*)nullptr));
 #pragma unroll
               for (int k = 0; k < DT; k += 2) {
                 uint32_t b[4];  // units k and k + 1, each keys 0-7 and 8-15
@@ -778,7 +800,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                 }
               }
             };
-            if (!near) add(__nv_bfloat16(), std::true_type());
+            if (__any_sync(0xffffffffu, far)) add(__nv_bfloat16(), std::true_type());
             else if (tail < 16) add(__half(), std::true_type());
             else add(__half(), std::false_type());
           }
@@ -805,12 +827,20 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+            if constexpr (Q8) {
+              // sums against z to sums against m (2^(z - m) by halves, which stay in fp32's range)
+              const float half = ex2_approx(0.5f * (z[nb][e] - m[nb][e]));
+#pragma unroll
+              for (int k = 0; k < DT; ++k) {
+                o[k][nb][e] = o[k][nb][e] * half * half;
+                o[k][nb][e + 2] = o[k][nb][e + 2] * half * half;
+              }
+            }
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], x);
             if (g == 0) mls[warp * ROWS + 8 * nb + 2 * t + e] = make_float2(m[nb][e], l[nb][e]);
           }
         meet();
-        const float v_up = Q8 && v_ref != 0.0f ? 1.0f / v_ref : 1.0f;
         float2 tot[RPW];   // of the rows this warp writes: warp, warp + WARPS, ...
         float acc[RPW][D / 32];
 #pragma unroll
@@ -837,8 +867,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                 for (int k = 0; k < DT; ++k)
 #pragma unroll
                   for (int h = 0; h < 2; ++h)
-                    mine[merge_at<D>(8 * nb + 2 * t + e, 16 * k + (Q8 ? 2 * g + h : g + 8 * h))] =
-                        o[k][nb][e + 2 * h] * v_up;
+                    mine[merge_at<D>(8 * nb + 2 * t + e, 16 * k + (Q8 ? 2 * g + h : g + 8 * h))] = o[k][nb][e + 2 * h];
           }
           meet();
 #pragma unroll

@@ -77,6 +77,10 @@ __device__ __forceinline__ float ldf<__nv_bfloat16>(const __nv_bfloat16* p) { re
 __device__ __forceinline__ float e8m0_to_float(uint32_t b) {
   return __uint_as_float(b == 0 ? 0x00400000u : b == 255 ? 0x7fffffffu : b << 23);
 }
+// b - 127, its exponent (NaN for 255).
+__device__ __forceinline__ float e8m0_exponent(uint32_t b) {
+  return b == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(0x4b000000u | b) - 8388735.0f;  // (2^23 + b) - ...
+}
 __device__ __forceinline__ void stf(float* p, float v) { *p = v; }
 __device__ __forceinline__ void stf(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void stf(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }

@@ -244,9 +244,9 @@ CMPX_API int cmpx_attention_select_path(int dtype, const void* Q, const void* K,
  * Softmax statistics and sums are fp32; the output is rounded once.  fp16 /
  * bf16 with head_dim 64 or 128 run tensor-core kernels (a flash-decoding
  * kernel for few query rows per kv head, a tcgen05 kernel for more; softmax
- * weights are rounded to 16 bits once, to bf16's where the scales of an 8-bit
- * cache's values differ by more than 2^6 up or 2^10 down from a block's first
- * ones).  They take pages of 8, 16, 32, ... keys (8-bit caches: 16, 32, ...,
+ * weights are rounded to 16 bits once; the flash-decoding kernel rounds them
+ * to fp16 over an 8-bit cache, to bf16 for 16 keys at a time that have a value
+ * scale 2^10 and more below those of a row's weightiest keys).  They take pages of 8, 16, 32, ... keys (8-bit caches: 16, 32, ...,
  * with contiguous scales of a page), 16-byte aligned addresses and strides of
  * 16-byte multiples.  fp32, other head_dim up to 512 and other layouts run a
  * CUDA-core kernel, which is correct but slow.  Values of an 8-bit cache are

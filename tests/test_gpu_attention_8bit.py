@@ -1,0 +1,200 @@
+"""attention_paged over e4m3 caches whose scales, pages and values are unusual,
+on every kernel, against the definition in 64 bits.
+
+Bound, besides seq_reference's: an output element is a sum of weight * code
+products, and a weight held in fp16 is off by at most half a step of its own
+(2^-11 relative) or, below 2^-14, by 2^-25.  The reference point of a row's
+weights lies at or below its largest weight (the tcgen05 kernel's) or its
+largest product of weight and scale 2^e (flash decoding's), so in units of the
+result the second part is at most
+
+    2^-25 * (max_j w_j * sum_j |v_j|  +  max_j w_j 2^e_j * sum_j |code_j|)
+
+over the visible keys.  Where the scales that a row meets lie more than 2^10
+below its largest product, flash decoding holds weights in bf16 (2^-8)."""
+import contextlib
+import math
+
+import pytest
+import torch
+
+import cabi
+import cmp_ext_b200 as cx
+from seq_reference import U, attend, check, e8m0, quantise
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+KERNELS = ["simt", "tc", "skinny"]
+
+
+@contextlib.contextmanager
+def forced(path):
+    cx._set_path(path)
+    try:
+        yield
+    finally:
+        cx._set_path("auto")
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+class Cache:
+    """One sequence in an e4m3 cache, pages in a random order; codes and scale
+    bytes of keys and values [length, hkv, d] / [length, hkv] are the caller's."""
+
+    def __init__(self, k, v, page=16, seed=0):
+        self.k, self.v, self.page = k, v, page  # (codes in 64 bits, bytes)
+        length, hkv, d = k[0].shape
+        need = -(-length // page)
+        order = torch.randperm(need + 2, generator=gen(seed), device="cuda")[:need]
+        self.table = order.int().view(1, need)
+        self.lens = torch.tensor([length], dtype=torch.int32, device="cuda")
+        j = torch.arange(length, device="cuda")
+        held = []
+        for codes, byte in (k, v):
+            c = torch.full((need + 2, hkv, page, d), math.nan, device="cuda")
+            s = torch.full((need + 2, hkv, page), 255, dtype=torch.uint8, device="cuda")
+            c[order[j // page], :, j % page] = codes.float()
+            s[order[j // page], :, j % page] = byte
+            held += [c.to(E4M3), s.view(E8M0)]
+        self.kc, self.ks, self.vc, self.vs = held
+
+    def lose(self, pages):
+        """These pages of the sequence are none: their keys and values are zeros."""
+        for p in pages:
+            self.table[0, p] = -1 if p % 2 else 10**6
+            for codes, byte in (self.k, self.v):
+                codes[p * self.page : (p + 1) * self.page] = 0
+                byte[p * self.page : (p + 1) * self.page] = 127
+
+    def run(self, q, **kw):
+        return cx.attention_paged(q, self.kc, self.vc, self.table, self.lens, key_scale=self.ks, value_scale=self.vs, **kw)
+
+    def check(self, got, q, what, u_w, scale=None):
+        n, hq, d = q.shape
+        length, hkv = self.k[1].shape
+        scale = 1 / math.sqrt(d) if scale is None else scale
+        kk, vv = (read_as(c, b, q.dtype) for c, b in (self.k, self.v))
+        want, tol = attend(q, kk, vv, scale, True, u_w, U[q.dtype])
+        step = 2.0**-25 if q.dtype == F16 else 2.0**-134  # half of the output's smallest
+        for i in range(n):
+            lim = max(0, min(length, length - n + i + 1))
+            if lim == 0:
+                continue
+            s = torch.einsum("hd,jhd->hj", q[i].double(), kk[:lim].repeat_interleave(hq // hkv, 1)) * scale
+            w = torch.softmax(s, -1)
+            e = torch.exp2(self.v[1][:lim].double() - 127).repeat_interleave(hq // hkv, 1).t()
+            e = torch.where(self.v[1][:lim].repeat_interleave(hq // hkv, 1).t() == 255, 0.0, e)
+            codes = self.v[0][:lim].double().nan_to_num().abs().sum(0).repeat_interleave(hq // hkv, 0)
+            vals = vv[:lim].nan_to_num().abs().sum(0).repeat_interleave(hq // hkv, 0)
+            tol[i] += step + 2.0**-25 * (w.amax(-1, keepdim=True) * vals + (w * e).amax(-1, keepdim=True) * codes)
+        check(got, want, tol, what)
+
+
+def read_as(codes, byte, dtype):
+    """What the cache holds in the queries' type: rounded to it, held to its finite range."""
+    x = codes.double() * e8m0(byte).unsqueeze(-1)
+    top = torch.finfo(dtype).max
+    return x.clamp(-top, top).to(dtype).double()
+
+
+def normal(length, hkv, d, seed):
+    """Codes and bytes of unit-normal vectors."""
+    return quantise(torch.randn(length, hkv, d, generator=gen(seed), device="cuda"))
+
+
+def scaled(length, hkv, d, bytes_, seed):
+    """Codes of full size with these scale bytes."""
+    codes, _ = quantise(torch.randn(length, hkv, d, generator=gen(seed), device="cuda"))
+    return codes, bytes_.to(torch.uint8).cuda().view(length, 1).expand(length, hkv).contiguous()
+
+
+def queries(n, hq, d, dtype, seed=1):
+    return torch.randn(n, hq, d, generator=gen(seed), device="cuda").to(dtype)
+
+
+def finish():
+    torch.cuda.synchronize()
+    assert cabi.device_error() == 0
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [1, 24])
+@pytest.mark.parametrize("lost", [[0], [3], [0, 1, 2, 3, 4, 5, 6], [12], range(0, 13, 2), range(13)])
+def test_pages_that_are_none(cuda, lost, n, dtype, path):
+    """Table entries that name no page read as zeros, wherever they lie."""
+    c = Cache(normal(200, 2, 64, 1), normal(200, 2, 64, 2))
+    c.lose(lost)
+    q = queries(n, 4, 64, dtype)
+    with forced(path):
+        out = c.run(q)
+    finish()
+    c.check(out, q, f"lost {list(lost)}", U[dtype])
+    if len(lost) == 13:
+        assert not out.any()
+
+
+def ramp(low, high, length):
+    return torch.linspace(low + 127, high + 127, length).round()
+
+
+SCALES = {
+    "rising": lambda x: ramp(-127, 100, x),
+    "falling": lambda x: ramp(100, -127, x),
+    "one first strip of 2^-127": lambda x: torch.where(torch.arange(x) < 16, 0, 120),
+    "one last key of 2^100": lambda x: torch.where(torch.arange(x) == x - 1, 227, 120),
+    "one first key of 2^100": lambda x: torch.where(torch.arange(x) == 0, 227, 120),
+    "in turn": lambda x: torch.tensor([7, 127, 200])[torch.arange(x) % 3],
+    "random": lambda x: torch.randint(0, 228, (x,), generator=torch.Generator().manual_seed(3)),
+}
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("n", [1, 24])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scales", list(SCALES))
+def test_value_scales_far_apart(cuda, scales, d, n, path):
+    """Every scale a byte can name, in any order along a sequence."""
+    length = 333
+    c = Cache(normal(length, 2, d, 3), scaled(length, 2, d, SCALES[scales](length), 4))
+    q = queries(n, 8, d, BF16)
+    with forced(path):
+        out = c.run(q)
+    finish()
+    c.check(out, q, scales, U[BF16])
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("n", [1, 24])
+@pytest.mark.parametrize("at", [0, 40, 199])
+def test_zero_vectors_beside_tiny_values(cuda, at, n, path):
+    """A vector of zeros has the scale 1, which lies far above that of values near 1e-10."""
+    length = 200
+    codes, byte = quantise(torch.randn(length, 2, 64, generator=gen(5), device="cuda") * 1e-10)
+    codes[at], byte[at] = 0, 127
+    c = Cache(normal(length, 2, 64, 6), (codes, byte))
+    q = queries(n, 4, 64, BF16)
+    with forced(path):
+        out = c.run(q)
+    finish()
+    c.check(out, q, f"zeros at {at}", U[BF16])
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("n", [1, 24])
+@pytest.mark.parametrize("length", [40, 1000])
+def test_weights_of_fp16_queries(cuda, length, n, path):
+    """Ordinary scales cost fp16 queries no more than fp16's own half step."""
+    x = torch.randn(length, 2, 128, generator=gen(7), device="cuda")
+    x *= 2.0 ** torch.randint(-2, 3, (length, 2, 1), generator=gen(8), device="cuda")
+    c = Cache(normal(length, 2, 128, 9), quantise(x))
+    q = queries(n, 8, 128, F16)
+    with forced(path):
+        out = c.run(q)
+    finish()
+    c.check(out, q, "fp16", U[F16])
