@@ -1,0 +1,72 @@
+"""Padded batches: tokens outside every sequence, as a captured call has them.
+Their rows are zeros in a new output, whatever the allocator left there, and
+cost about what writing them costs."""
+import math
+
+import pytest
+import torch
+
+import cabi
+import cmp_ext_b200 as cx
+from seq_reference import U, attend, check
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def cu(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def qkv(tokens, hq, hkv, d, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(tokens, hq + 2 * hkv, d, generator=g, device="cuda").to(dtype)
+    return x[:, :hq], x[:, hq : hq + hkv], x[:, hq + hkv :]
+
+
+@pytest.mark.parametrize("path", ["tc", "skinny", "simt"])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (7, 1, 128), (128, 1, 64), (6, 2, 64)])
+@pytest.mark.parametrize("first,used,total", [(0, 300, 1500), (700, 130, 1001), (5, 0, 777), (900, 1, 901)])
+def test_rows_outside_are_zeros(cuda, first, used, total, hq, hkv, d, path):
+    q, k, v = qkv(total, hq, hkv, d, BF16, total)
+    at = cu(first, first + used)
+    size = total * hq * d
+    junk = torch.full((size,), math.nan, dtype=BF16, device="cuda")  # what the next allocation of that size gets
+    cx._set_path(path)
+    try:
+        del junk
+        out = cx.attention_varlen(q, k, v, at)
+    finally:
+        cx._set_path("auto")
+    torch.cuda.synchronize()
+    assert cabi.device_error() == 0
+    assert not out[:first].any() and not out[first + used :].any()
+    sees = slice(first, first + min(used, 40))
+    rows = out[sees]
+    want, tol = attend(q[sees], k[sees], v[sees], 1 / math.sqrt(d), True, U[BF16], U[BF16])
+    check(rows, want, tol, "the sequence")
+
+
+@pytest.mark.parametrize("total,used", [(16384, 300), (65536, 64)])
+def test_padding_costs_what_writing_it_costs(cuda, total, used):
+    q, k, v = qkv(total, 32, 8, 128, BF16, 1)
+    at = cu(0, used)
+
+    def best(f):
+        times = []
+        for _ in range(7):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            f()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    out = torch.empty(total, 32, 128, dtype=BF16, device="cuda")
+    written = best(lambda: out.zero_())
+    whole = best(lambda: cx.attention_varlen(q, k, v, at))
+    alone = best(lambda: cx.attention_varlen(q, k, v, at, out=out))  # rows outside are left as they were
+    print(f"{total} tokens, {used} used: {whole:.3f} ms, {alone:.3f} without zeros, writing zeros {written:.3f}")
+    assert whole <= alone + 4 * written + 0.05
