@@ -41,21 +41,24 @@
 // An 8-bit cache runs in fp16, where its codes are exact.  bf16 queries are
 // brought into fp16's range by a power of two a row (exact for magnitudes down
 // to 2^-31 of the row's largest), and key scales multiply the scores in fp32.
-// Value scales 2^e join the exponent of the weights that multiply the codes,
-// 2^(s + e - z), against a reference point z of their own, which a row moves
-// like that of its scores: whatever the scales of the keys it sees, in whatever
-// order, these weights stay below 2^8 and its largest one near 2^2, while the
-// sum of 2^(s - m) keeps its own bits; 2^(z - m) joins the two when a piece
-// ends.  A reference shared by the rows of a warp or taken once would let a
-// later, larger scale overflow.  Where a key's scale lies 2^10 and more below
-// z - m (a vector of zeros, whose scale is 1, among tiny ones puts z that high),
-// fp16 might drop its bits: the strip takes bf16 weights, whose range is fp32's.
+// Value scales 2^e multiply the weights: 2^(s - m) 2^(e - d) goes with the
+// codes, d a reference of each row that follows the largest s + e of the keys
+// it sees; o 2^d is what the sum of 2^(s - m) divides.  As long as scales stay
+// within 2^-10 .. 2^6 of every row's 2^d (the warp's band), these weights stay
+// below 2^14 and one multiplication by an exact power of two is all that takes.
+// A strip that leaves the band, or holds values that the queries' type does not
+// (tiny ones, or beyond its largest), moves d where a row's weight calls for it
+// and is summed key by key in fp32, where no scale overflows or loses bits.
+// That path is kept short: inlined as products of converted values it made
+// the loop slower for strips that do not take it (48 x 3 bf16 tokens of 32 / 8
+// heads of 128 over 1000 to 24000 keys: 234 us, this way 207).
 //
 // Values that are not finite: as in attention_tile.cu, a row whose result is
 // not finite although its sum is, and that may not see one of them, is
 // computed again over its visible keys.
 #include <cuda_fp8.h>
 
+#include <climits>
 #include <type_traits>
 
 #include "attention_math.cuh"
@@ -71,6 +74,7 @@ constexpr float kNone = -3.4028234663852886e38f;  // reference point of a row wi
 struct DecodeParams {
   SeqProblem p;
   int box_rows;     // keys of one TMA box
+  int box_lg;       // log2 of them
   int blocks;       // most blocks that share the work
   int whole;        // no unit is split: a block takes whole ones, and no second kernel runs
   int rows;         // of a unit: 8 or 16
@@ -106,6 +110,8 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d of 2^-d.
+__device__ __forceinline__ float row_exponent(float r) { return float(127 - int(__float_as_uint(r) >> 23)); }
 // An 8 x 8 matrix of 16-bit values, turned.
 __device__ __forceinline__ uint32_t turn8x8(uint32_t a) {
   uint32_t d;
@@ -186,6 +192,7 @@ constexpr int kEnds = 1;     // the piece's last tile
 constexpr int kWhole = 2;    // the piece is the whole unit
 constexpr int kFirst = 4;    // the unit begins in this block
 constexpr int kLast = 8;     // the block's last tile
+constexpr int kMissing = 8;  // from this bit on: boxes of the tile (16 at most) whose page is none, 8-bit caches
 
 // Query row r of a unit: its token, head, and visible keys (0: no such row).
 struct Row {
@@ -229,45 +236,6 @@ struct DecodeCfg {
 template <int D>
 __device__ __forceinline__ int merge_at(int r, int d) {
   return r * D + (d ^ ((r >> 1 & 3) << 3));
-}
-
-// One row over keys [kbeg, kend) from its definition; a warp computes it.
-template <typename T, int D, bool Q8>
-__device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk, const T* q, int kbeg, int kend,
-                                      float m, float (&acc)[D / 32]) {
-  const int lane = threadIdx.x & 31;
-  constexpr int NV = D / 32;
-  using KV = typename std::conditional<Q8, __nv_fp8_e4m3, T>::type;
-  auto load = [](const KV* at) -> float {
-    if constexpr (Q8) return float(*at);
-    else return ldf(at);
-  };
-#pragma unroll
-  for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
-  for (int j = kbeg; j < kend; ++j) {
-    int64_t ko = int64_t(k0 + j) * p.k.row, vo = int64_t(k0 + j) * p.v.row;
-    float ks = 1.0f, vs = 1.0f;
-    if (p.table != nullptr) {
-      const int page = __ldg(p.table + b * p.table_stride + j / p.page_size), slot = j % p.page_size;
-      if (page < 0 || page >= p.pages) continue;  // zeros
-      ko = page * p.k.page + slot * p.k.row;
-      vo = page * p.v.page + slot * p.v.row;
-      if (Q8) {
-        ks = e8m0_to_float(p.k.scale[page * p.k.s_page + hk * p.k.s_head + slot * p.k.s_row]);
-        vs = e8m0_to_float(p.v.scale[page * p.v.s_page + hk * p.v.s_head + slot * p.v.s_row]);
-      }
-    }
-    const KV* kr = static_cast<const KV*>(p.k.base) + ko + hk * p.k.head;
-    const KV* vr = static_cast<const KV*>(p.v.base) + vo + hk * p.v.head;
-    float dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) dot = fmaf(ldf(q + lane + 32 * i), load(kr + lane + 32 * i), dot);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float w = ex2_approx(dot * ks * p.scale_log2 - m) * vs;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] = fmaf(w, load(vr + lane + 32 * i), acc[i]);
-  }
 }
 
 template <int FMT, int D, bool Q8, int NB>
@@ -453,7 +421,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
         ok = false;
         break;
       }
-      // scales of pages that are none: zeros, as TMA gives for their codes
+      // pages that are none: TMA gives zeros for their codes; keys' scales 1,
+      // values' 2^-127, which no band takes and a multiplication makes 0
       const bool there = lane < boxes && now >= 0 && now < p.pages;
       uint32_t bytes = uint32_t(max(boxes, 0) * a.box_rows * Cfg::ROW * 2);
       if constexpr (Q8) {
@@ -461,7 +430,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
           for (int k = 0; k < a.box_rows; k += 4)
 #pragma unroll
             for (int v = 0; v < 2; ++v)
-              *reinterpret_cast<uint32_t*>(scales + st * Cfg::SCALES + v * KEYS + lane * a.box_rows + k) = 0u;
+              *reinterpret_cast<uint32_t*>(scales + st * Cfg::SCALES + v * KEYS + lane * a.box_rows + k) =
+                  v ? 0u : 0x7f7f7f7fu;
+        info.flags |= int(__ballot_sync(0xffffffffu, lane < boxes && !there)) << kMissing;
         bytes += uint32_t(__popc(__ballot_sync(0xffffffffu, there)) * a.box_rows * 2);
       }
       __syncwarp();
@@ -522,6 +493,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       else return base ^ (2 * i << 4);
     };
     constexpr int PITCH = Cfg::ROW < 128 ? 64 : 128;
+    // 8-bit code of strip row j, column d (the swizzle of lane_at)
+    auto code_at = [](const uint8_t* base, int j, int d) -> const uint8_t* {
+      return base + j * PITCH + (((d >> 4) ^ (PITCH == 64 ? j >> 1 & 3 : j & 7)) << 4) + (d & 15);
+    };
     int strip = warp;                     // the next of this warp's strips, counted from the tile's first
     int st = 0, flags = busy ? 0 : kLast;
     uint32_t phase = 0, join_phase = 0;
@@ -551,7 +526,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       uint32_t qf[DT][NB][2];               // Q^T: row g of block nb
       float o[DT][NB][4];                   // O^T: two columns, rows 2t and 2t + 1
       float m[NB][2], l[NB][2], qs[NB][2];  // rows 2t, 2t + 1: reference point, sum (this lane's keys), score factor
-      float z[NB][2];                       // 8-bit: reference point of the weights that multiply the codes
+      float rs[NB][2];                      // 8-bit: 2^-d of the rows
+      uint32_t band = 256, band_n = 0;      // 8-bit: the value scale bytes band .. band + band_n are within it (none)
       int lim[NB][2];
       int lim_min;                          // of all rows
       {
@@ -603,9 +579,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
           lim_min = min(lim_min, __reduce_min_sync(0xffffffffu, keys));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            qs[nb][e] = p.scale_log2 * __shfl_sync(0xffffffffu, up, 4 * (2 * t + e));
+            qs[nb][e] = FMT == 1 && Q8 ? p.scale_log2 * __shfl_sync(0xffffffffu, up, 4 * (2 * t + e)) : p.scale_log2;
             lim[nb][e] = __shfl_sync(0xffffffffu, keys, 4 * (2 * t + e));
-            m[nb][e] = z[nb][e] = kNone;
+            m[nb][e] = kNone;
+            rs[nb][e] = 1.0f;
             l[nb][e] = 0.0f;
           }
         }
@@ -655,28 +632,36 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
               }
             }
           }
-          const uint8_t* sc = scales + st * Cfg::SCALES + strip * 16 + g;
-          float ks[2] = {1.0f, 1.0f}, ve[2] = {0.0f, 0.0f};  // scales of keys, exponents of those of values
+          const uint8_t* sc = scales + st * Cfg::SCALES + strip * 16;
+          const uint8_t* kstrip = ring + size_t(st) * 2 * HALF + strip * 16 * PITCH;  // (8-bit) its codes
+          float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};  // scales of keys and values g and g + 8
+          // 8-bit: the strip holds a value scale out of the band, or a key that
+          // fp16 does not (bf16's range is fp32's but for its last half step)
+          bool odd = false;
           if constexpr (Q8) {
-            ks[0] = e8m0_to_float(sc[0]);
-            ks[1] = e8m0_to_float(sc[8]);
-            ve[0] = e8m0_exponent(sc[KEYS]);
-            ve[1] = e8m0_exponent(sc[KEYS + 8]);
+            bool is[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t kb = sc[g + 8 * h], vb = sc[KEYS + g + 8 * h];
+              ks[h] = FMT == 0 ? __uint_as_float(kb << 23) : e8m0_to_float(kb);  // (right unless odd)
+              vs[h] = __uint_as_float(vb << 23);
+              is[h] = vb - band > band_n || (FMT == 0 && !scale4_takes(kb, (T*)nullptr));
+            }
+            if (tail < 16) {  // what lies behind the last key may be anything
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (g + 8 * h >= tail) {
+                  vs[h] = 0.0f;
+                  is[h] = false;
+                }
+            }
+            odd = is[0] || is[1];
           }
           // in log2 units; hidden scores -inf
-          float s[NB][4], c[NB][4];  // c (8-bit): exponents of the weights that multiply the codes
+          float s[NB][4];
           bool grew = false;
           const bool cut = kv0 + 16 > lim_min;
-          // (behind s, since a hidden value's scale may be a NaN)
-          auto code_exponents = [&](int nb) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[nb][e] = s[nb][e] - z[nb][e & 1] + ve[e >> 1];
-            if (cut) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]) c[nb][e] = -INFINITY;
-            }
-          };
+          auto hidden = [&](int nb, int e) -> bool { return cut && kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]; };
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -687,57 +672,144 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
             if (cut) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (kv0 + g + 8 * (e >> 1) >= lim[nb][e & 1]) s[nb][e] = -INFINITY;
+                if (hidden(nb, e)) s[nb][e] = -INFINITY;
             }
             grew = grew || fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kGrow || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kGrow;
-            if constexpr (Q8) {
-              code_exponents(nb);
-              grew = grew || fmaxf(fmaxf(c[nb][0], c[nb][1]), fmaxf(c[nb][2], c[nb][3])) > kGrow;
-            }
           }
-          if (__any_sync(0xffffffffu, grew)) {
+          bool exact = false;  // 8-bit: the strip is summed key by key
+          float ve[2] = {0.0f, 0.0f};
+          if (__any_sync(0xffffffffu, grew || odd)) {
+            if constexpr (Q8) {
+              const int keys = flags >> (kMissing + (strip * 16 >> a.box_lg)) & 1 ? 0 : tail;
+              uint32_t vb[2];
+              bool live[2], strange = false;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+              for (int h = 0; h < 2; ++h) {
+                live[h] = g + 8 * h < keys;
+                vb[h] = sc[KEYS + g + 8 * h];
+                ve[h] = e8m0_exponent(vb[h]);
+                strange = strange || (FMT == 0 && live[h] && !scale4_takes(sc[g + 8 * h], (T*)nullptr));
+              }
+              if (FMT == 0 && __any_sync(0xffffffffu, strange)) {
+                // the scores of keys as T holds them, one by one
+#pragma unroll 1
+                for (int j = 0; j < min(keys, 16); ++j) {
+                  const float up = e8m0_to_float(sc[j]);
+                  float dot[NB];  // of row g of a block, this lane's columns
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float mx = fmaxf(s[nb][e], s[nb][e + 2]);
+                  for (int nb = 0; nb < NB; ++nb) dot[nb] = 0.0f;
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                const bool up = mx > m[nb][e] + kGrow;
-                const float m_new = up ? mx - kBias : m[nb][e];
-                float alpha = up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
-                m[nb][e] = m_new;
-                l[nb][e] *= alpha;
-                if constexpr (Q8) {
-                  float high = -INFINITY;  // largest score + exponent (hidden ones, -inf and NaN left out)
+                  for (int k = 0; k < DT; ++k) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(code_at(kstrip, j, 16 * k + 4 * t));
 #pragma unroll
-                  for (int h = 0; h < 2; ++h)
-                    if (c[nb][e + 2 * h] > -INFINITY) high = fmaxf(high, s[nb][e + 2 * h] + ve[h]);
+                    for (int e = 0; e < 2; ++e) {
+                      const uint32_t two = dequant2(e ? w >> 16 : w & 0xffffu, up, (T*)nullptr);
+                      const float a0 = ldf(reinterpret_cast<const T*>(&two)), a1 = ldf(reinterpret_cast<const T*>(&two) + 1);
 #pragma unroll
-                  for (int x = 4; x < 32; x <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
-                  const float z_new = high > z[nb][e] + kGrow ? high - kBias : z[nb][e];
-                  alpha = z_new != z[nb][e] ? ex2_approx(z[nb][e] - z_new) : 1.0f;
-                  z[nb][e] = z_new;
-                }
+                      for (int nb = 0; nb < NB; ++nb) {
+                        uint32_t two_q = qf[k][nb][e];
+                        asm volatile("" : "+r"(two_q));  // (converted here, not ahead of the loop: that spills)
+                        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&two_q));
+                        dot[nb] = fmaf(x.y, a1, fmaf(x.x, a0, dot[nb]));
+                      }
+                    }
+                  }
 #pragma unroll
-                for (int k = 0; k < DT; ++k) {
-                  o[k][nb][e] *= alpha;
-                  o[k][nb][e + 2] *= alpha;
+                  for (int nb = 0; nb < NB; ++nb) {
+                    dot[nb] += __shfl_xor_sync(0xffffffffu, dot[nb], 1);
+                    dot[nb] += __shfl_xor_sync(0xffffffffu, dot[nb], 2);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                      const float x = __shfl_sync(0xffffffffu, dot[nb], 4 * (2 * t + e)) * qs[nb][e];
+#pragma unroll
+                      for (int h = 0; h < 2; ++h)
+                        if (j == g + 8 * h) s[nb][e + 2 * h] = hidden(nb, e + 2 * h) ? -INFINITY : x;
+                    }
+                  }
                 }
               }
-            if constexpr (Q8) {
+              int d_min = INT_MAX, d_max = INT_MIN;  // of rows that have seen a key
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) code_exponents(nb);
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float mx = fmaxf(s[nb][e], s[nb][e + 2]);
+#pragma unroll
+                  for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                  const bool up = mx > m[nb][e] + kGrow;
+                  const float m_new = up ? mx - kBias : m[nb][e];
+                  const float d = row_exponent(rs[nb][e]);
+                  // largest exponent of a visible key's weight times scale, and
+                  // whether one beyond the band has a weight that d must follow
+                  // (-inf and NaN drop out of both; pages that are none do not count)
+                  float high = -INFINITY;
+                  bool over = false;
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    if (!live[h] || hidden(nb, e + 2 * h)) continue;
+                    const float c = s[nb][e + 2 * h] - m_new + ve[h];
+                    high = fmaxf(high, c);
+                    over = over || (ve[h] - d > 6.0f && c - d > kGrow);
+                  }
+                  over = over || up;
+#pragma unroll
+                  for (int x = 4; x < 32; x <<= 1) {
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
+                    over = __shfl_xor_sync(0xffffffffu, int(over), x) != 0 || over;
+                  }
+                  const float top = fmaxf(m[nb][e] - m_new + d, high - kBias);
+                  const float d_new = over ? fminf(fmaxf(rintf(top), -120.0f), 120.0f) : d;
+                  const float alpha = over ? ex2_approx(m[nb][e] - m_new + (d - d_new)) : 1.0f;
+                  l[nb][e] *= up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
+                  m[nb][e] = m_new;
+                  rs[nb][e] = __uint_as_float(uint32_t(127 - int(d_new)) << 23);
+                  if (m_new != kNone) {
+                    d_min = min(d_min, int(d_new));
+                    d_max = max(d_max, int(d_new));
+                  }
+#pragma unroll
+                  for (int k = 0; k < DT; ++k) {
+                    o[k][nb][e] *= alpha;
+                    o[k][nb][e + 2] *= alpha;
+                  }
+                }
+              d_min = __reduce_min_sync(0xffffffffu, d_min);
+              d_max = __reduce_max_sync(0xffffffffu, d_max);
+              const int from = max(d_max + 117, FMT == 0 ? 113 : 1), to = min(d_min + 133, FMT == 0 ? 134 : 245);
+              const bool some = d_min <= d_max && from <= to;
+              band = some ? uint32_t(from) : 256u;
+              band_n = some ? uint32_t(to - from) : 0u;
+              exact = __any_sync(0xffffffffu, (live[0] && vb[0] - band > band_n) || (live[1] && vb[1] - band > band_n));
+            } else {
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float mx = fmaxf(s[nb][e], s[nb][e + 2]);
+#pragma unroll
+                  for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                  const bool up = mx > m[nb][e] + kGrow;
+                  const float m_new = up ? mx - kBias : m[nb][e];
+                  const float alpha = up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
+                  m[nb][e] = m_new;
+                  l[nb][e] *= alpha;
+#pragma unroll
+                  for (int k = 0; k < DT; ++k) {
+                    o[k][nb][e] *= alpha;
+                    o[k][nb][e + 2] *= alpha;
+                  }
+                }
             }
           }
-          bool far = false;  // 8-bit: a visible key's scale lies 2^10 and more below z - m
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if constexpr (Q8) far = far || (ve[e >> 1] <= z[nb][e & 1] - m[nb][e & 1] - 10.0f && c[nb][e] > -INFINITY);
-              s[nb][e] = ex2_approx(s[nb][e] - m[nb][e & 1]);
-              l[nb][e & 1] += s[nb][e];
+              const float x = s[nb][e] - m[nb][e & 1], w = ex2_approx(x);
+              l[nb][e & 1] += w;
+              s[nb][e] = Q8 ? w * (vs[e >> 1] * rs[nb][e & 1]) : w;
+              if (Q8 && exact)  // (w may be 0 where the scale makes up for it)
+                s[nb][e] = hidden(nb, e) ? 0.0f : ex2_approx(x + (ve[e >> 1] - row_exponent(rs[nb][e & 1])));
             }
           // ---- O^T += V^T P^T.  Value rows behind the last key may hold
           // anything: their elements are cleared
@@ -767,18 +839,12 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
             if (tail < 16) add(std::true_type());
             else add(std::false_type());
           } else {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) c[nb][e] = ex2_approx(c[nb][e]);
-            auto add = [&](auto half_type, auto clear) {
-              using P = decltype(half_type);
-              constexpr bool kBf = std::is_same<P, __nv_bfloat16>::value;
+            auto add = [&](auto clear) {
               uint32_t pf[NB][2];
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(c[nb][2 * h], c[nb][2 * h + 1], (P*)nullptr));
+                for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (__half*)nullptr));
 #pragma unroll
               for (int k = 0; k < DT; k += 2) {
                 uint32_t b[4];  // units k and k + 1, each keys 0-7 and 8-15
@@ -790,19 +856,44 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                   uint32_t f[4];
                   e4m3_to_half(__byte_perm(b[2 * u], 0, 0x3120), f[0], f[1]);
                   e4m3_to_half(__byte_perm(b[2 * u + 1], 0, 0x3120), f[2], f[3]);
+                  if constexpr (decltype(clear)::value) {
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    if constexpr (kBf) f[e] = half2_to_bf16(f[e]);
-                    if constexpr (decltype(clear)::value) f[e] &= keep(e >> 1);
+                    for (int e = 0; e < 4; ++e) f[e] &= keep(e >> 1);
                   }
 #pragma unroll
-                  for (int nb = 0; nb < NB; ++nb) mma16<kBf>(o[k + u][nb], f, pf[nb][0], pf[nb][1]);
+                  for (int nb = 0; nb < NB; ++nb) mma16<false>(o[k + u][nb], f, pf[nb][0], pf[nb][1]);
                 }
               }
             };
-            if (__any_sync(0xffffffffu, far)) add(__nv_bfloat16(), std::true_type());
-            else if (tail < 16) add(__half(), std::true_type());
-            else add(__half(), std::false_type());
+            if (exact) {
+#pragma unroll 1
+              for (int j = 0; j < min(tail, 16); ++j) {
+                float w[NB][2];  // of key j, rows 2t and 2t + 1
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    w[nb][e] = __shfl_sync(0xffffffffu, j < 8 ? s[nb][e] : s[nb][e + 2], 4 * (j & 7) + t);
+                const CodeScale by = code_scale(sc[KEYS + j]);
+#pragma unroll
+                for (int k = 0; k < DT; ++k) {
+                  const uint32_t codes2 = *reinterpret_cast<const uint16_t*>(code_at(kstrip + HALF, j, 16 * k + 2 * g));
+                  const uint32_t two = dequant2(codes2, by.up, (T*)nullptr);
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const float v = ldf(reinterpret_cast<const T*>(&two) + h) * by.down;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                      for (int e = 0; e < 2; ++e) o[k][nb][e + 2 * h] = fmaf(w[nb][e], v, o[k][nb][e + 2 * h]);
+                  }
+                }
+              }
+            } else if (tail < 16) {
+              add(std::true_type());
+            } else {
+              add(std::false_type());
+            }
           }
         }
         strip -= KEYS / 16;
@@ -828,12 +919,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             if constexpr (Q8) {
-              // sums against z to sums against m (2^(z - m) by halves, which stay in fp32's range)
-              const float half = ex2_approx(0.5f * (z[nb][e] - m[nb][e]));
+              // times 2^d; and against m + kBias, for which a single key has
+              // the weight 1: its value may be the largest there is
+              m[nb][e] += kBias;
+              l[nb][e] *= ex2_approx(-kBias);
+              const float up = ex2_approx(-kBias) * __uint_as_float((254u - (__float_as_uint(rs[nb][e]) >> 23)) << 23);
 #pragma unroll
               for (int k = 0; k < DT; ++k) {
-                o[k][nb][e] = o[k][nb][e] * half * half;
-                o[k][nb][e + 2] = o[k][nb][e + 2] * half * half;
+                o[k][nb][e] *= up;
+                o[k][nb][e + 2] *= up;
               }
             }
 #pragma unroll
@@ -1067,6 +1161,7 @@ cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, int 
   a.rows = rows;
   a.keys = decode_keys(p, q8);
   a.box_rows = paged && p.page_size < a.keys ? p.page_size : a.keys;
+  while ((2 << a.box_lg) <= a.box_rows) ++a.box_lg;
   a.whole = decode_whole(p);
   if (a.whole) {
     // a block a unit, up to a few waves

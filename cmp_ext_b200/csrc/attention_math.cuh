@@ -6,6 +6,7 @@
 #include <cuda_fp8.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace cmpx {
 
@@ -85,6 +86,8 @@ __device__ __forceinline__ void stf(float* p, float v) { *p = v; }
 __device__ __forceinline__ void stf(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void stf(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// What an 8-bit cache holds is the same to every kernel: code * 2^e rounded to
+// the queries' type T, beyond its largest value that value.
 // Two e4m3 codes times a scale, in T, saturating.
 __device__ __forceinline__ uint32_t dequant2(uint32_t codes, float up, __half*) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes), __NV_E4M3);
@@ -99,6 +102,17 @@ __device__ __forceinline__ uint32_t dequant2(uint32_t codes, float up, __nv_bflo
   uint32_t r;
   asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y * up), "f"(f.x * up));
   return r;
+}
+// One code, as a float (T = float: nothing to round to but fp32).
+template <typename T>
+__device__ __forceinline__ float held(uint32_t code, float up) {
+  if constexpr (sizeof(T) == 4) {
+    const float x = __half2float(__half(__nv_cvt_fp8_to_halfraw(__nv_fp8_storage_t(code), __NV_E4M3))) * up;
+    return x > 3.4028234663852886e38f ? 3.4028234663852886e38f : x < -3.4028234663852886e38f ? -3.4028234663852886e38f : x;
+  } else {
+    const uint16_t one = uint16_t(dequant2(code, up, (T*)nullptr) & 0xffffu);
+    return ldf(reinterpret_cast<const T*>(&one));
+  }
 }
 
 // Four e4m3 codes as two fp16 pairs (exact): codes 0 and 1, codes 2 and 3.
@@ -138,6 +152,17 @@ __device__ __forceinline__ void scale4(uint32_t codes, uint32_t byte, uint32_t& 
                        y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), s);
   lo = *reinterpret_cast<const uint32_t*>(&x);
   hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+
+// For kernels that multiply codes and keep the scale 2^e outside:
+// held(code, up) * down is the code whose product with 2^e T holds.
+struct CodeScale {
+  float up, down;  // 2^e, 2^-e
+};
+__device__ __forceinline__ CodeScale code_scale(uint32_t byte) {
+  if (byte == 255) return CodeScale{1.0f, 1.0f};  // (the NaN stays outside)
+  return CodeScale{e8m0_to_float(byte), e8m0_to_float(254u - byte)};
 }
 
 }  // namespace cmpx

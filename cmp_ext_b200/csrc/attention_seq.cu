@@ -1,8 +1,6 @@
 // Attention over packed sequences and paged caches (cmpx_attention_seq):
 // argument checks, path selection and the CUDA-core kernel.  No counterpart
 // in the reference.
-#include <cuda_fp8.h>
-
 #include <climits>
 
 #include "attention_math.cuh"
@@ -11,12 +9,12 @@
 namespace cmpx {
 namespace {
 
-// Scalar loads of keys and values; an 8-bit code's scale is applied by the
-// caller, to the score or to the weight.
-__device__ __forceinline__ float ldkv(const float* p) { return *p; }
-__device__ __forceinline__ float ldkv(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ float ldkv(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float ldkv(const __nv_fp8_e4m3* p) { return float(*p); }
+// Scalar loads of keys and values; `up` an 8-bit code's scale.
+template <typename T, typename KV>
+__device__ __forceinline__ float ldkv(const KV* p, float up) {
+  if constexpr (sizeof(KV) == 1) return held<T>(*p, up);
+  else return ldf(p);
+}
 
 // Sequence that holds token t (the last one that begins at or before it), or
 // -1 for a token of none.
@@ -90,11 +88,11 @@ __global__ void __launch_bounds__(128) attention_seq_simt_kernel(const SeqProble
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int d = lane + 32 * i;
-      if (there && d < p.d) dot = fmaf(qv[i], ldkv(kb + ko + d), dot);
+      if (there && d < p.d) dot = fmaf(qv[i], ldkv<T>(kb + ko + d, ks), dot);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float x = dot * ks * p.scale_log2;
+    const float x = dot * p.scale_log2;
     const float m_new = fmaxf(m, x);
     const float m_use = m_new == -INFINITY ? 0.0f : m_new;  // nothing finite so far: all weights 0
     const float alpha = exp2f(m - m_use);
@@ -104,7 +102,7 @@ __global__ void __launch_bounds__(128) attention_seq_simt_kernel(const SeqProble
     for (int i = 0; i < NV; ++i) {
       const int d = lane + 32 * i;
       acc[i] *= alpha;
-      if (there && d < p.d) acc[i] = fmaf(w * vs, ldkv(vb + vo + d), acc[i]);
+      if (there && d < p.d) acc[i] = fmaf(w, ldkv<T>(vb + vo + d, vs), acc[i]);
     }
     m = m_new;
   }
@@ -289,9 +287,9 @@ bool seq_kv_maps(const SeqProblem& p, int kv_dtype, int box_rows, bool swizzled,
 
 cudaError_t launch_seq_simt(const SeqProblem& p, int dtype, int kv_dtype, cudaStream_t s) {
   if (kv_dtype == CMPX_E4M3)
-    return dtype == CMPX_F16    ? launch_simt_typed<__half, __nv_fp8_e4m3>(p, s)
-           : dtype == CMPX_BF16 ? launch_simt_typed<__nv_bfloat16, __nv_fp8_e4m3>(p, s)
-                                : launch_simt_typed<float, __nv_fp8_e4m3>(p, s);
+    return dtype == CMPX_F16    ? launch_simt_typed<__half, uint8_t>(p, s)
+           : dtype == CMPX_BF16 ? launch_simt_typed<__nv_bfloat16, uint8_t>(p, s)
+                                : launch_simt_typed<float, uint8_t>(p, s);
   return dtype == CMPX_F16    ? launch_simt_typed<__half, __half>(p, s)
          : dtype == CMPX_BF16 ? launch_simt_typed<__nv_bfloat16, __nv_bfloat16>(p, s)
                               : launch_simt_typed<float, float>(p, s);

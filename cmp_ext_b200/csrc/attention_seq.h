@@ -2,7 +2,9 @@
 // (attention_seq.cu: checks, dispatch, CUDA-core kernel).
 #pragma once
 #include <cstdint>
+#include <type_traits>
 
+#include "attention_math.cuh"
 #include "internal.h"
 
 namespace cmpx {
@@ -100,6 +102,46 @@ __device__ __forceinline__ bool seq_hidden_bad(const SeqProblem& p, int b, int k
     }
   }
   return __any_sync(0xffffffffu, bad);
+}
+// One row over keys [kbeg, kend) of a sequence from its definition: the sums
+// of weights 2^(x - m) times values.  A warp computes it, lane i the columns
+// i, i + 32, ...
+template <typename T, int D, bool Q8>
+__device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk, const T* q, int kbeg, int kend,
+                                         float m, float (&acc)[D / 32]) {
+  const int lane = threadIdx.x & 31;
+  constexpr int NV = D / 32;
+  using KV = typename std::conditional<Q8, uint8_t, T>::type;
+  auto load = [](const KV* at, float up) -> float {
+    if constexpr (Q8) return held<T>(*at, up);
+    else return ldf(at);
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
+  for (int j = kbeg; j < kend; ++j) {
+    int64_t ko = int64_t(k0 + j) * p.k.row, vo = int64_t(k0 + j) * p.v.row;
+    float ks = 1.0f, vs = 1.0f;
+    if (p.table != nullptr) {
+      const int page = __ldg(p.table + b * p.table_stride + j / p.page_size), slot = j % p.page_size;
+      if (page < 0 || page >= p.pages) continue;  // reads as zeros: nothing to add
+      ko = page * p.k.page + slot * p.k.row;
+      vo = page * p.v.page + slot * p.v.row;
+      if (Q8) {
+        ks = e8m0_to_float(p.k.scale[page * p.k.s_page + hk * p.k.s_head + slot * p.k.s_row]);
+        vs = e8m0_to_float(p.v.scale[page * p.v.s_page + hk * p.v.s_head + slot * p.v.s_row]);
+      }
+    }
+    const KV* kr = static_cast<const KV*>(p.k.base) + ko + hk * p.k.head;
+    const KV* vr = static_cast<const KV*>(p.v.base) + vo + hk * p.v.head;
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) dot = fmaf(ldf(q + lane + 32 * i), load(kr + lane + 32 * i, ks), dot);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    const float w = ex2_approx(fmaf(dot, p.scale_log2, -m));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = fmaf(w, load(vr + lane + 32 * i, vs), acc[i]);
+  }
 }
 // First token that no sequence holds any more (cu_seqlens_q[batch], clamped),
 // and the number of tokens before the first sequence.

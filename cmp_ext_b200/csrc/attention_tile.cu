@@ -101,66 +101,6 @@ __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// One row from its definition: keys [kbeg, kend) of sequence s / head hk,
-// weights 2^(x - m).  A warp computes it, lane d the columns d, d + 32, ...
-// final_row: the output row, divided by l; else part_row gets the sums.
-template <typename T, int D, bool Q8>
-__device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk, const T* q, int kbeg, int kend,
-                                      float m, float inv, T* final_row, float* part_row) {
-  const int lane = threadIdx.x & 31;
-  constexpr int NV = D / 32;
-  using KV = typename std::conditional<Q8, __nv_fp8_storage_t, T>::type;
-  float qv[NV], acc[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    qv[i] = ldf(q + lane + 32 * i);
-    acc[i] = 0.0f;
-  }
-  for (int j = kbeg; j < kend; ++j) {
-    int64_t ko, vo;
-    float ks = 1.0f, vs = 1.0f;
-    if (p.table != nullptr) {
-      const int page = __ldg(p.table + b * p.table_stride + j / p.page_size), slot = j % p.page_size;
-      if (page < 0 || page >= p.pages) {  // reads as zeros: a score of 0, a value of 0
-        continue;
-      }
-      ko = page * p.k.page + slot * p.k.row;
-      vo = page * p.v.page + slot * p.v.row;
-      if (Q8) {
-        ks = e8m0_to_float(p.k.scale[page * p.k.s_page + hk * p.k.s_head + slot * p.k.s_row]);
-        vs = e8m0_to_float(p.v.scale[page * p.v.s_page + hk * p.v.s_head + slot * p.v.s_row]);
-      }
-    } else {
-      ko = int64_t(k0 + j) * p.k.row;
-      vo = int64_t(k0 + j) * p.v.row;
-    }
-    const KV* kr = static_cast<const KV*>(p.k.base) + ko + hk * p.k.head;
-    const KV* vr = static_cast<const KV*>(p.v.base) + vo + hk * p.v.head;
-    auto load = [&](const KV* at, float up) -> float {
-      if constexpr (Q8) {
-        const uint32_t two = dequant2(*at, up, (T*)nullptr);
-        const uint16_t one = uint16_t(two & 0xffffu);
-        return ldf(reinterpret_cast<const T*>(&one));
-      } else {
-        return ldf(at);
-      }
-    };
-    float dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) dot = fmaf(qv[i], load(kr + lane + 32 * i, ks), dot);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float w = ex2_approx(fmaf(dot, p.scale_log2, -m));
-#pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] = fmaf(w, load(vr + lane + 32 * i, vs), acc[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (final_row != nullptr) stf(final_row + lane + 32 * i, acc[i] * inv);
-    else part_row[lane + 32 * i] = acc[i];
-  }
-}
-
 // Zeros in the rows that no sequence holds, heads of kv head hk: this block's
 // share of them over the grid's x axis, by `threads` threads.  A padded batch
 // has far more such rows than others, and blocks without a tile then: those
@@ -786,7 +726,13 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
         float* pf = a.splits > 1 ? a.part_o + (int64_t(blockIdx.z) * p.tokens_q * p.heads_q +
                                                int64_t(s.q0 + tok) * p.heads_q + hd) * D
                                  : nullptr;
-        redo_row<T, D, Q8>(p, seq, s.k0, hk, q, jb * 128, kl, mm, ii, a.splits > 1 ? nullptr : of, pf);
+        float acc[D / 32];
+        redo_row<T, D, Q8>(p, seq, s.k0, hk, q, jb * 128, kl, mm, acc);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          if (a.splits > 1) pf[lane + 32 * i] = acc[i];
+          else stf(of + lane + 32 * i, acc[i] * ii);
+        }
       }
     }
   }

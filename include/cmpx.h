@@ -245,12 +245,14 @@ CMPX_API int cmpx_attention_select_path(int dtype, const void* Q, const void* K,
  * bf16 with head_dim 64 or 128 run tensor-core kernels (a flash-decoding
  * kernel for few query rows per kv head, a tcgen05 kernel for more; softmax
  * weights are rounded to 16 bits once; the flash-decoding kernel rounds them
- * to fp16 over an 8-bit cache, to bf16 for 16 keys at a time that have a value
- * scale 2^10 and more below those of a row's weightiest keys).  They take pages of 8, 16, 32, ... keys (8-bit caches: 16, 32, ...,
+ * to fp16 over an 8-bit cache, and not at all where value scales lie far apart).  They take pages of 8, 16, 32, ... keys (8-bit caches: 16, 32, ...,
  * with contiguous scales of a page), 16-byte aligned addresses and strides of
  * 16-byte multiples.  fp32, other head_dim up to 512 and other layouts run a
- * CUDA-core kernel, which is correct but slow.  Values of an 8-bit cache are
- * taken in the queries' type, held to its finite range.
+ * CUDA-core kernel, which is correct but slow.  Keys and values of an 8-bit
+ * cache are to every kernel what cmpx_kv_cache_read gives in the queries' type:
+ * code * 2^e rounded to it, beyond its largest finite value that value.  (Of
+ * bf16's range flash decoding leaves out the ends: parts of a 2^-133 below
+ * normal values, and a key that e4m3 rounds up to 2^128 stays that.)
  *
  * All strides are in elements.  The element stride within a head is 1. */
 typedef struct {

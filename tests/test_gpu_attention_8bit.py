@@ -10,8 +10,7 @@ result the second part is at most
 
     2^-25 * (max_j w_j * sum_j |v_j|  +  max_j w_j 2^e_j * sum_j |code_j|)
 
-over the visible keys.  Where the scales that a row meets lie more than 2^10
-below its largest product, flash decoding holds weights in bf16 (2^-8)."""
+over the visible keys."""
 import contextlib
 import math
 
@@ -198,3 +197,72 @@ def test_weights_of_fp16_queries(cuda, length, n, path):
         out = c.run(q)
     finish()
     c.check(out, q, "fp16", U[F16])
+
+
+BEYOND = {  # exponents of scales along a sequence, in turn
+    "above": [5, 9, 12, 40, 127],
+    "below": [-15, -20, -26, -33, -60, -127],
+    "both": [-7, 9, -20, 100, -127, 3],
+    "one above": [-7] * 40 + [9],
+    "one below": [-7] * 40 + [-16],
+}
+
+
+def in_turn(exponents, length):
+    return torch.tensor(exponents)[torch.arange(length) % len(exponents)] + 127
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("n,length", [(1, 150), (24, 150), (3, 7)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scales", list(BEYOND))
+def test_values_beyond_fp16(cuda, scales, d, n, length, path):
+    """What a cache holds of larger and of smaller vectors than fp16 does is
+    taken as fp16 has it, as kv_cache_read gives it: on every kernel."""
+    c = Cache(normal(length, 2, d, 10), scaled(length, 2, d, in_turn(BEYOND[scales], length), 11))
+    q = queries(n, 8, d, F16)
+    with forced(path):
+        out = c.run(q)
+    finish()
+    c.check(out, q, scales, U[F16])
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("n,length", [(1, 150), (24, 150), (3, 7)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scales", list(BEYOND))
+def test_keys_beyond_fp16(cuda, scales, d, n, length, path):
+    c = Cache(scaled(length, 2, d, in_turn(BEYOND[scales], length), 12), normal(length, 2, d, 13))
+    scale = 0.2 if scales in ("below", "one below") else 1e-5
+    q = queries(n, 8, d, F16)
+    with forced(path):
+        out = c.run(q, scale=scale)
+    finish()
+    c.check(out, q, scales, U[F16], scale)
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_the_largest_value(cuda, dtype, path):
+    """e4m3 rounds the types' largest values up to a power of two beyond them;
+    read back they are the largest ones again, and a row that sees one key
+    gives its value."""
+    if dtype == F32 and path != "simt":
+        pytest.skip("not this kernel's")
+    top = torch.finfo(dtype).max
+    v = torch.full((1, 2, 64), top, dtype=dtype, device="cuda")
+    v[:, :, ::2] *= -1
+    kc, vc = (torch.zeros(2, 2, 16, 64, device="cuda").to(E4M3) for _ in range(2))
+    ks, vs = (torch.zeros(2, 2, 16, dtype=torch.uint8, device="cuda").view(E8M0) for _ in range(2))
+    cx.kv_cache_write(torch.ones_like(v), v, kc, vc, torch.tensor([19], device="cuda"), ks, vs)
+    table, lens = torch.tensor([[1]], dtype=torch.int32, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda")
+    # the first three tokens' values are zeros of the smallest scale; their keys give -inf of weight
+    kc[1, :, :3] = torch.full((2, 3, 64), -448.0, device="cuda").to(E4M3)
+    ks.view(torch.uint8)[1, :, :3] = 127
+    q = torch.full((1, 4, 64), 8.0, dtype=dtype, device="cuda")
+    with forced(path):
+        out = cx.attention_paged(q, kc, vc, table, lens, key_scale=ks, value_scale=vs)
+    finish()
+    read = cx.kv_cache_read(kc, vc, torch.tensor([19], device="cuda"), ks, vs, dtype=dtype)[1]
+    assert torch.equal(read, v)
+    assert torch.equal(out, v.repeat_interleave(2, 1))
