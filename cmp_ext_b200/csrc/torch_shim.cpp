@@ -438,7 +438,6 @@ std::pair<const char*, const char*> span_of(const torch::Tensor& t) {
 bool overlaps(const std::pair<const char*, const char*>& x, const std::pair<const char*, const char*>& y) {
   return x.first < x.second && y.first < y.second && x.first < y.second && y.first < x.second;
 }
-bool overlaps(const torch::Tensor& a, const torch::Tensor& b) { return overlaps(span_of(a), span_of(b)); }
 
 // A tensor that a kernel writes in place: unit stride along D, and no two
 // elements on one address.
@@ -456,31 +455,59 @@ void check_writable(const torch::Tensor& t, const char* name, bool unit_last) {
   }
 }
 
-// Whether `delta` elements lie between two places of a tensor with these
-// (stride, size) pairs, largest stride first, none of whose elements share an
-// address.
-bool reaches(const std::vector<std::pair<int64_t, int64_t>>& dims, size_t i, int64_t delta) {
-  if (i == dims.size()) return delta == 0;
-  const int64_t stride = dims[i].first, most = dims[i].second - 1;
-  const int64_t down = delta >= 0 ? delta / stride : -((-delta + stride - 1) / stride);
-  for (int64_t d : {down, down + 1})
-    if (d >= -most && d <= most && reaches(dims, i + 1, delta - d * stride)) return true;
+// A strided tensor as runs of bytes: (stride, size) in bytes of what repeats
+// them, largest stride first.
+struct Runs {
+  const char* base;
+  int64_t run;
+  c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;
+  c10::SmallVector<int64_t, 5> span;  // bytes from the first to the last, of dims[i ...]
+};
+Runs runs_of(const torch::Tensor& t) {
+  Runs r{static_cast<const char*>(t.data_ptr()), t.element_size(), {}, {}};
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) > 0) r.dims.emplace_back(t.stride(i) * t.element_size(), t.size(i));
+  std::sort(r.dims.begin(), r.dims.end(), [](const auto& x, const auto& y) { return x > y; });
+  while (!r.dims.empty() && r.dims.back().first <= r.run) {  // what lies side by side is one run
+    r.run += r.dims.back().first * (r.dims.back().second - 1);
+    r.dims.pop_back();
+  }
+  r.span.assign(r.dims.size() + 1, r.run);
+  for (size_t i = r.dims.size(); i-- > 0;) r.span[i] = r.span[i + 1] + r.dims[i].first * (r.dims[i].second - 1);
+  return r;
+}
+
+// Whether a's dims [i ...] from x on and b's [j ...] from y on share a byte.
+// Only repetitions whose ranges meet are looked into; those of one stride in
+// both (a buffer's pages, say) count by their distance.  Layouts that would
+// take too many steps count as sharing one.
+bool runs_meet(const Runs& a, size_t i, const char* x, const Runs& b, size_t j, const char* y, int& steps) {
+  if (x >= y + b.span[j] || y >= x + a.span[i]) return false;
+  const bool more_a = i < a.dims.size(), more_b = j < b.dims.size();
+  if ((!more_a && !more_b) || --steps < 0) return true;
+  if (more_a && more_b && a.dims[i].first == b.dims[j].first) {
+    // x + d * stride + [0, span of a's rest) meets y + [0, span of b's rest)
+    const int64_t stride = a.dims[i].first, gap = y - x;
+    const int64_t low = -(b.dims[j].second - 1), high = a.dims[i].second - 1;
+    for (int64_t d = std::max(low, (gap - a.span[i + 1]) / stride - 1); d <= high && d * stride < gap + b.span[j + 1]; ++d)
+      if (runs_meet(a, i + 1, x + d * stride, b, j + 1, y, steps)) return true;
+    return false;
+  }
+  if (!more_a || (more_b && b.dims[j].first > a.dims[i].first)) return runs_meet(b, j, y, a, i, x, steps);
+  const int64_t stride = a.dims[i].first, gap = y - x;
+  for (int64_t d = std::max<int64_t>(0, (gap - a.span[i + 1]) / stride - 1);
+       d < a.dims[i].second && d * stride < gap + b.span[j]; ++d)
+    if (runs_meet(a, i + 1, x + d * stride, b, j, y, steps)) return true;
   return false;
 }
 
-// Two tensors that a kernel writes together (both passed check_writable) share
-// an element.  Views of one buffer may lie between each other's rows if they
-// have the same layout; with different ones their ranges must be apart.
+// Two tensors share a byte (views of one buffer may lie between each other's
+// rows).
 bool share_elements(const torch::Tensor& a, const torch::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0 || !overlaps(a, b)) return false;
-  if (a.sizes() != b.sizes() || a.strides() != b.strides() || a.element_size() != b.element_size()) return true;
-  const int64_t bytes = static_cast<const char*>(a.data_ptr()) - static_cast<const char*>(b.data_ptr());
-  if (bytes % a.element_size() != 0) return true;
-  std::vector<std::pair<int64_t, int64_t>> dims;
-  for (int64_t i = 0; i < a.dim(); ++i)
-    if (a.size(i) > 1) dims.emplace_back(a.stride(i), a.size(i));
-  std::sort(dims.rbegin(), dims.rend());
-  return reaches(dims, 0, bytes / a.element_size());
+  if (a.numel() == 0 || b.numel() == 0 || !overlaps(span_of(a), span_of(b))) return false;
+  const Runs x = runs_of(a), y = runs_of(b);
+  int steps = 20000;
+  return runs_meet(x, 0, x.base, y, 0, y.base, steps);
 }
 
 // query / key / value as the kernels take them: unit stride along D, and for
@@ -516,7 +543,7 @@ torch::Tensor seq_output(const c10::optional<torch::Tensor>& out, const torch::T
   TORCH_CHECK(out->device() == query.device(), "Device mismatch");
   check_writable(*out, "out", true);
   for (const torch::Tensor* t : inputs)
-    if (t != nullptr && t->defined()) TORCH_CHECK(!overlaps(*out, *t), "out must not overlap an input");
+    if (t != nullptr && t->defined()) TORCH_CHECK(!share_elements(*out, *t), "out must not overlap an input");
   return *out;
 }
 
@@ -773,7 +800,8 @@ void kv_cache_write(torch::Tensor key, torch::Tensor value, torch::Tensor key_ca
     written[2] = {&*key_scale, "key_scale", {}};
     written[3] = {&*value_scale, "value_scale", {}};
   }
-  const std::pair<const char*, const char*> inputs[3] = {span_of(key), span_of(value), span_of(slots)};
+  const std::pair<const torch::Tensor*, std::pair<const char*, const char*>> inputs[3] = {
+      {&key, span_of(key)}, {&value, span_of(value)}, {&slots, span_of(slots)}};
   for (int i = 0; i < (kv == CMPX_E4M3 ? 4 : 2); ++i) {
     Written& w = written[i];
     check_writable(*w.t, w.name, i < 2);
@@ -781,7 +809,8 @@ void kv_cache_write(torch::Tensor key, torch::Tensor value, torch::Tensor key_ca
     for (int j = 0; j < i; ++j)
       TORCH_CHECK(!overlaps(w.span, written[j].span) || !share_elements(*w.t, *written[j].t), w.name, " must not be ",
                   written[j].name, " or overlap it");
-    for (const auto& in : inputs) TORCH_CHECK(!overlaps(w.span, in), w.name, " must not overlap an input");
+    for (const auto& in : inputs)
+      TORCH_CHECK(!overlaps(w.span, in.second) || !share_elements(*w.t, *in.first), w.name, " must not overlap an input");
   }
   TORCH_CHECK(key.is_cuda(), "kv_cache_write expects CUDA tensors");
   c10::cuda::CUDAGuard guard(key.device());
