@@ -79,6 +79,7 @@ struct DecodeParams {
   int whole;        // no unit is split: a block takes whole ones, and no second kernel runs
   int rows;         // of a unit: 8 or 16
   int keys;         // of a tile
+  int most;         // weight of the list that ascending offsets can make at most
   float* part_o;    // [blocks][2][rows][D]
   float2* part_ml;  // [blocks][2][rows]
   int* joints;      // [tokens_q][heads_q]: first block, pieces << 12, row of the unit << 24 (one piece: written)
@@ -133,6 +134,8 @@ __device__ __forceinline__ int unit_weight(const DecodeParams& a, int nt) { retu
 // Tile that place x of a unit's weight stands for: the first kUnitCost + 1
 // places are the first tile's.
 __device__ __forceinline__ int place_tile(const DecodeParams& a, int x) { return a.whole ? 0 : max(x - kUnitCost, 0); }
+// Sum of two weights, as far as an int goes.
+__device__ __forceinline__ int add_weight(int x, int y) { return int(min(uint32_t(x) + uint32_t(y), 0x7fffffffu)); }
 // First place of block c: floor(c * total / used).
 __device__ __forceinline__ int first_place(int c, int total, int used) {
   const int q = total / used;
@@ -292,15 +295,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += up;
+      if (lane >= o) upto = add_weight(upto, up);
     }
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
     int all = 0;
 #pragma unroll
     for (int w = 0; w <= WARPS; ++w) {
-      if (w == warp) upto += all;
-      all += warp_sum[w];
+      if (w == warp) upto = add_weight(upto, all);
+      all = add_weight(all, warp_sum[w]);
     }
     __syncthreads();
     return all;
@@ -308,8 +311,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
   int total = 0;
   for (int base = 0; base < p.batch; base += THREADS) {
     const int all = count_pass(base);
-    total += all;
+    total = add_weight(total, all);
   }
+  // offsets that do not ascend may name the same tokens many times: no work
+  // then (and no sum that an int cannot hold)
+  if (total > a.most) total = 0;
   const int used = min(total, a.blocks);
   // the places of its first tile and of the next block's
   const int c_id = int(blockIdx.x);
@@ -1102,6 +1108,13 @@ int64_t decode_blocks(const DeviceInfo& dev, int rows) { return int64_t(dev.num_
 // than the second kernel costs.
 bool decode_whole(const SeqProblem& p) { return (p.table != nullptr ? p.max_keys : p.tokens_kv) <= 512; }
 
+// More places than any lengths can make of the problem (64 keys, 8 rows each).
+double most_places(const SeqProblem& p) {
+  const double rows = double(p.tokens_q) * p.group / 8 + p.batch;
+  const double keys = double(p.table != nullptr ? p.max_keys : p.tokens_kv) / 64 + 1;
+  return rows * (keys + kUnitCost) * p.heads_kv;
+}
+
 template <int FMT, int D, bool Q8, int NB>
 cudaError_t launch_decode_rows(const DecodeParams& a, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t s) {
   using Cfg = DecodeCfg<D, Q8, NB>;
@@ -1135,17 +1148,10 @@ cudaError_t launch_decode_typed(const DecodeParams& a, const CUtensorMap& tk, co
 
 }  // namespace
 
-// More tiles than any lengths can make of the problem (64 keys, 8 rows each).
-double most_tiles(const SeqProblem& p) {
-  const double rows = double(p.tokens_q) * p.group / 8 + p.batch;
-  const double keys = double(p.table != nullptr ? p.max_keys : p.tokens_kv) / 64 + 1;
-  return rows * keys * p.heads_kv;
-}
-
 bool seq_decode_ok(const SeqProblem& p, int dtype, int kv_dtype) {
   return (dtype == CMPX_F16 || dtype == CMPX_BF16) && (p.d == 64 || p.d == 128) && seq_tma_ok(p, kv_dtype) &&
          seq_rows_ok(p.Q, p.q_token, p.tokens_q, 8) && seq_rows_ok(p.Q, p.q_head, p.heads_q, 8) &&
-         (int64_t(p.tokens_q) * p.heads_q + 3) / 4 <= 0x7fffffffLL && most_tiles(p) < 0x7fffffff;
+         (int64_t(p.tokens_q) * p.heads_q + 3) / 4 <= 0x7fffffffLL && most_places(p) < 0x7fffffff;
 }
 
 size_t seq_decode_workspace(const SeqProblem& p, int rows, const DeviceInfo& dev) {
@@ -1174,6 +1180,7 @@ cudaError_t launch_seq_decode(const SeqProblem& p, int dtype, int kv_dtype, int 
     a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(a.blocks) * 2 * rows * p.d);
     a.joints = reinterpret_cast<int*>(a.part_ml + int64_t(a.blocks) * 2 * rows);
   }
+  a.most = int(most_places(p));
   a.err = err;
   CUtensorMap tk, tv;
   if (!seq_kv_maps(p, kv_dtype, a.box_rows, true, &tk, &tv)) return cudaErrorInvalidValue;

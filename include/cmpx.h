@@ -290,7 +290,8 @@ typedef struct {
 
 /* Runs the packed (page_table NULL) or the paged form.  Lengths and page
  * numbers are read on the device: out-of-range ones are clamped, and a key
- * whose page number is outside [0, pages) reads as zeros. */
+ * whose page number is outside [0, pages) reads as zeros.  Offsets that do not
+ * ascend leave rows of O without a meaning, and nothing else. */
 CMPX_API int cmpx_attention_seq(const cmpx_attention_seq_args* args, cmpx_stream_t stream);
 
 /* Workspace bytes cmpx_attention_seq needs on the current device (partial

@@ -70,3 +70,32 @@ def test_padding_costs_what_writing_it_costs(cuda, total, used):
     alone = best(lambda: cx.attention_varlen(q, k, v, at, out=out))  # rows outside are left as they were
     print(f"{total} tokens, {used} used: {whole:.3f} ms, {alone:.3f} without zeros, writing zeros {written:.3f}")
     assert whole <= alone + 4 * written + 0.05
+
+
+@pytest.mark.parametrize("path", ["tc", "skinny", "simt"])
+@pytest.mark.parametrize("batch,width", [(9, 40), (400, 40), (100000, 1024)])
+def test_offsets_that_do_not_ascend(cuda, batch, width, path):
+    """The same 64 tokens named again and again, with more work in them than 32
+    bits count: no access outside, no endless call, and later calls are right."""
+    hq, hkv, d, page, t = 32, 8, 64, 64, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    kc, vc = (torch.randn(width, hkv, page, d, generator=g, device="cuda").to(F16) for _ in range(2))
+    q = torch.randn(t, hq, d, generator=g, device="cuda").to(F16)
+    table = torch.arange(width, dtype=torch.int32, device="cuda").view(1, width).expand(batch, width)
+    lens = torch.full((batch,), width * page, dtype=torch.int32, device="cuda")
+    at = torch.zeros(batch + 1, dtype=torch.int32, device="cuda")
+    at[1::2] = t
+    cx._set_path(path)
+    try:
+        cx.attention_paged(q, kc, vc, table, lens, cu_seqlens_q=at)
+        cx.attention_varlen(q, *(x.reshape(-1, hkv, d)[:t].contiguous() for x in (kc, vc)), at)
+        torch.cuda.synchronize()
+        assert cabi.device_error() == 0
+        out = cx.attention_paged(q[:3], kc, vc, table[:3, :2], torch.tensor([100, 5, 128], dtype=torch.int32, device="cuda"))
+    finally:
+        cx._set_path("auto")
+    torch.cuda.synchronize()
+    keys = kc[:2].transpose(1, 2).reshape(-1, hkv, d), vc[:2].transpose(1, 2).reshape(-1, hkv, d)
+    for i, n in enumerate((100, 5, 128)):
+        want, tol = attend(q[i : i + 1], keys[0][:n], keys[1][:n], 1 / math.sqrt(d), True, U[F16], U[F16])
+        check(out[i : i + 1], want, tol, f"row {i}")
