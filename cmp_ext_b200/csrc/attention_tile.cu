@@ -728,6 +728,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
                                  : nullptr;
         float acc[D / 32];
         redo_row<T, D, Q8>(p, seq, s.k0, hk, q, jb * 128, kl, mm, acc);
+        __syncwarp();  // behind the stores of the row's own thread, which these replace
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           if (a.splits > 1) pf[lane + 32 * i] = acc[i];
