@@ -432,12 +432,14 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       const bool there = lane < boxes && now >= 0 && now < p.pages;
       uint32_t bytes = uint32_t(max(boxes, 0) * a.box_rows * Cfg::ROW * 2);
       if constexpr (Q8) {
-        if (lane < boxes && !there)
+        if (lane < boxes && !there) {
           for (int k = 0; k < a.box_rows; k += 4)
 #pragma unroll
             for (int v = 0; v < 2; ++v)
               *reinterpret_cast<uint32_t*>(scales + st * Cfg::SCALES + v * KEYS + lane * a.box_rows + k) =
                   v ? 0u : 0x7f7f7f7fu;
+          fence_proxy_async_smem();  // before a later copy writes the place
+        }
         info.flags |= int(__ballot_sync(0xffffffffu, lane < boxes && !there)) << kMissing;
         bytes += uint32_t(__popc(__ballot_sync(0xffffffffu, there)) * a.box_rows * 2);
       }

@@ -329,8 +329,10 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
           uint32_t bytes = uint32_t(boxes * a.box_rows * D * (Q8 ? 1 : 2));
           uint8_t* sdst = sScale + ((2 * j + v) % RS) * 128 + lane * a.box_rows;
           if constexpr (Q8) {
-            if (lane < boxes && !there)
+            if (lane < boxes && !there) {
               for (int k = 0; k < a.box_rows; k += 4) *reinterpret_cast<uint32_t*>(sdst + k) = 0u;
+              fence_proxy_async_smem();  // before a later copy writes the place
+            }
             bytes += uint32_t(__popc(__ballot_sync(0xffffffffu, there)) * a.box_rows);
           }
           __syncwarp();
