@@ -817,11 +817,13 @@ cudaError_t launch_tile_typed(const TileParams& a, const CUtensorMap& tq, const 
   if (e != cudaSuccess) return e;
   // setmaxnreg.inc waits for registers of the block's own: the shares must fit
   // what the kernel was compiled to launch with
-  static int regs = 0;
+  static int known = 0;  // (threads may make their first calls at once)
+  int regs = __atomic_load_n(&known, __ATOMIC_RELAXED);
   if (regs == 0) {
     cudaFuncAttributes fa = {};
     if ((e = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return e;
     regs = fa.numRegs;
+    __atomic_store_n(&known, regs, __ATOMIC_RELAXED);
   }
   if (Cfg::WARPS / 4 * regs < Cfg::REGS_NEED) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
