@@ -42,16 +42,20 @@
 // brought into fp16's range by a power of two a row (exact for magnitudes down
 // to 2^-31 of the row's largest), and key scales multiply the scores in fp32.
 // Value scales 2^e multiply the weights: 2^(s - m) 2^(e - d) goes with the
-// codes, d a reference of each row that follows the largest s + e of the keys
-// it sees; o 2^d is what the sum of 2^(s - m) divides.  As long as scales stay
-// within 2^-10 .. 2^6 of every row's 2^d (the warp's band), these weights stay
-// below 2^14 and one multiplication by an exact power of two is all that takes.
-// A strip that leaves the band, or holds values that the queries' type does not
-// (tiny ones, or beyond its largest), moves d where a row's weight calls for it
-// and is summed key by key in fp32, where no scale overflows or loses bits.
-// That path is kept short: inlined as products of converted values it made
-// the loop slower for strips that do not take it (48 x 3 bf16 tokens of 32 / 8
-// heads of 128 over 1000 to 24000 keys: 234 us, this way 207).
+// codes, and o 2^d is what the sum of 2^(s - m) divides.  d = c + shift: c of
+// each row follows the largest s + e of the keys it sees, so that no scale
+// overflows whatever order they come in; the warp's shift (40 either way) follows
+// the scales of a strip.  As long as these stay within 2^-10 .. 2^6 of every
+// row's 2^d (the warp's band), weights stay below 2^14, keep fp16's bits down to
+// 2^-4, and one multiplication by an exact power of two is all that takes.  A
+// strip that leaves the band moves it; one that fits into no band (scales 2^16
+// apart, rows that are) has its weights in two bf16 parts, 16 bits in fp32's
+// range.  A strip with values beyond the largest of the queries' type, which
+// are that value to every kernel, is summed key by key in fp32: rare, and kept
+// out of the way of the others (products of converted values inlined in the
+// loop made 48 x 3 bf16 tokens of 32 / 8 heads over 1000 to 24000 keys take 234
+// us, this way 212).  Scales of 14 binades at random make 48 single tokens take
+// 202 us instead of 122, where key by key it would be 690.
 //
 // Values that are not finite: as in attention_tile.cu, a row whose result is
 // not finite although its sum is, and that may not see one of them, is
@@ -250,6 +254,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
   constexpr bool BF = FMT == 1 && !Q8;  // the products' type
   constexpr int KEYS = Cfg::KEYS, STAGES = Cfg::STAGES, HALF = Cfg::HALF, WARPS = Cfg::WARPS, THREADS = Cfg::THREADS;
   constexpr int DT = D / 16;            // 16-wide steps of q . k, 16-wide tiles of the output
+  // largest scale byte whose codes (448 at most) stay within T's range
+  constexpr uint32_t kTopScale = FMT == 0 ? 134 : 245;
   const SeqProblem& p = a.p;
 
   extern __shared__ uint8_t smem_raw[];
@@ -536,6 +542,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
       float m[NB][2], l[NB][2], qs[NB][2];  // rows 2t, 2t + 1: reference point, sum (this lane's keys), score factor
       float rs[NB][2];                      // 8-bit: 2^-d of the rows
       uint32_t band = 256, band_n = 0;      // 8-bit: the value scale bytes band .. band + band_n are within it (none)
+      int shift = 0;                        // 8-bit: d - c of all rows
       int lim[NB][2];
       int lim_min;                          // of all rows
       {
@@ -644,7 +651,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
           const uint8_t* kstrip = ring + size_t(st) * 2 * HALF + strip * 16 * PITCH;  // (8-bit) its codes
           float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};  // scales of keys and values g and g + 8
           // 8-bit: the strip holds a value scale out of the band, or a key that
-          // fp16 does not (bf16's range is fp32's but for its last half step)
+          // may be beyond fp16's largest value (bf16's is fp32's but for half a step)
           bool odd = false;
           if constexpr (Q8) {
             bool is[2];
@@ -653,7 +660,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
               const uint32_t kb = sc[g + 8 * h], vb = sc[KEYS + g + 8 * h];
               ks[h] = FMT == 0 ? __uint_as_float(kb << 23) : e8m0_to_float(kb);  // (right unless odd)
               vs[h] = __uint_as_float(vb << 23);
-              is[h] = vb - band > band_n || (FMT == 0 && !scale4_takes(kb, (T*)nullptr));
+              is[h] = vb - band > band_n || (FMT == 0 && kb > kTopScale);
             }
             if (tail < 16) {  // what lies behind the last key may be anything
 #pragma unroll
@@ -663,7 +670,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                   is[h] = false;
                 }
             }
-            odd = is[0] || is[1];
+            // (a page that is none holds zeros, whatever its scales)
+            odd = !(flags >> (kMissing + (strip * 16 >> a.box_lg)) & 1) && (is[0] || is[1]);
           }
           // in log2 units; hidden scores -inf
           float s[NB][4];
@@ -684,21 +692,23 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
             }
             grew = grew || fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kGrow || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kGrow;
           }
-          bool exact = false;  // 8-bit: the strip is summed key by key
+          // 8-bit: a strip out of the band; one with values beyond T's largest
+          bool exact = false, beyond = false;
           float ve[2] = {0.0f, 0.0f};
           if (__any_sync(0xffffffffu, grew || odd)) {
             if constexpr (Q8) {
               const int keys = flags >> (kMissing + (strip * 16 >> a.box_lg)) & 1 ? 0 : tail;
               uint32_t vb[2];
-              bool live[2], strange = false;
+              bool live[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 live[h] = g + 8 * h < keys;
                 vb[h] = sc[KEYS + g + 8 * h];
                 ve[h] = e8m0_exponent(vb[h]);
-                strange = strange || (FMT == 0 && live[h] && !scale4_takes(sc[g + 8 * h], (T*)nullptr));
+                beyond = beyond || (live[h] && vb[h] > kTopScale);
               }
-              if (FMT == 0 && __any_sync(0xffffffffu, strange)) {
+              beyond = __any_sync(0xffffffffu, beyond);
+              if (FMT == 0 && __any_sync(0xffffffffu, (live[0] && sc[g] > kTopScale) || (live[1] && sc[g + 8] > kTopScale))) {
                 // the scores of keys as T holds them, one by one
 #pragma unroll 1
                 for (int j = 0; j < min(keys, 16); ++j) {
@@ -736,7 +746,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                   }
                 }
               }
-              int d_min = INT_MAX, d_max = INT_MIN;  // of rows that have seen a key
+              // scale exponents of the strip, and of the rows that have seen a key
+              int v_min = INT_MAX, v_max = INT_MIN, c_min = INT_MAX, c_max = INT_MIN;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (live[h] && vb[h] != 255) {
+                  v_min = min(v_min, int(vb[h]) - 127);
+                  v_max = max(v_max, int(vb[h]) - 127);
+                }
+              float by[NB][2];  // exponent that the sums of a row get
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -746,18 +764,18 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                   for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                   const bool up = mx > m[nb][e] + kGrow;
                   const float m_new = up ? mx - kBias : m[nb][e];
-                  const float d = row_exponent(rs[nb][e]);
+                  const float d = row_exponent(rs[nb][e]), c_old = d - float(shift);
                   // largest exponent of a visible key's weight times scale, and
-                  // whether one beyond the band has a weight that d must follow
+                  // whether one beyond the band has a weight that c must follow
                   // (-inf and NaN drop out of both; pages that are none do not count)
                   float high = -INFINITY;
                   bool over = false;
 #pragma unroll
                   for (int h = 0; h < 2; ++h) {
                     if (!live[h] || hidden(nb, e + 2 * h)) continue;
-                    const float c = s[nb][e + 2 * h] - m_new + ve[h];
-                    high = fmaxf(high, c);
-                    over = over || (ve[h] - d > 6.0f && c - d > kGrow);
+                    const float x = s[nb][e + 2 * h] - m_new + ve[h];
+                    high = fmaxf(high, x);
+                    over = over || (ve[h] - d > 6.0f && x - c_old > kGrow);
                   }
                   over = over || up;
 #pragma unroll
@@ -765,28 +783,44 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, x));
                     over = __shfl_xor_sync(0xffffffffu, int(over), x) != 0 || over;
                   }
-                  const float top = fmaxf(m[nb][e] - m_new + d, high - kBias);
-                  const float d_new = over ? fminf(fmaxf(rintf(top), -120.0f), 120.0f) : d;
-                  const float alpha = over ? ex2_approx(m[nb][e] - m_new + (d - d_new)) : 1.0f;
+                  const float top = fmaxf(m[nb][e] - m_new + c_old, high - kBias);
+                  const float c_new = over ? fminf(fmaxf(rintf(top), -80.0f), 80.0f) : c_old;
                   l[nb][e] *= up ? ex2_approx(m[nb][e] - m_new) : 1.0f;
+                  by[nb][e] = m[nb][e] - m_new + d - c_new;
                   m[nb][e] = m_new;
-                  rs[nb][e] = __uint_as_float(uint32_t(127 - int(d_new)) << 23);
+                  rs[nb][e] = c_new;  // (2^-d below)
                   if (m_new != kNone) {
-                    d_min = min(d_min, int(d_new));
-                    d_max = max(d_max, int(d_new));
+                    c_min = min(c_min, int(c_new));
+                    c_max = max(c_max, int(c_new));
                   }
+                }
+              v_min = __reduce_min_sync(0xffffffffu, v_min);
+              v_max = __reduce_max_sync(0xffffffffu, v_max);
+              c_min = __reduce_min_sync(0xffffffffu, c_min);
+              c_max = __reduce_max_sync(0xffffffffu, c_max);
+              const bool some = c_min <= c_max;
+              if (!some) c_min = c_max = 0;
+              auto fits = [&](int x) -> bool { return c_max + x - 10 <= v_min && c_min + x + 6 >= v_max; };
+              if (some && v_min <= v_max && !fits(shift)) {
+                const int to = max(-40, min(40, v_max - c_max));
+                if (fits(to)) shift = to;
+              }
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int d = int(rs[nb][e]) + shift;
+                  const float alpha = ex2_approx(by[nb][e] - float(shift));
+                  rs[nb][e] = __uint_as_float(uint32_t(127 - d) << 23);
 #pragma unroll
                   for (int k = 0; k < DT; ++k) {
                     o[k][nb][e] *= alpha;
                     o[k][nb][e + 2] *= alpha;
                   }
                 }
-              d_min = __reduce_min_sync(0xffffffffu, d_min);
-              d_max = __reduce_max_sync(0xffffffffu, d_max);
-              const int from = max(d_max + 117, FMT == 0 ? 113 : 1), to = min(d_min + 133, FMT == 0 ? 134 : 245);
-              const bool some = d_min <= d_max && from <= to;
-              band = some ? uint32_t(from) : 256u;
-              band_n = some ? uint32_t(to - from) : 0u;
+              const int from = max(c_max + shift + 117, 1), to = min(c_min + shift + 133, int(kTopScale));
+              band = some && from <= to ? uint32_t(from) : 256u;
+              band_n = some && from <= to ? uint32_t(to - from) : 0u;
               exact = __any_sync(0xffffffffu, (live[0] && vb[0] - band > band_n) || (live[1] && vb[1] - band > band_n));
             } else {
 #pragma unroll
@@ -847,12 +881,20 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
             if (tail < 16) add(std::true_type());
             else add(std::false_type());
           } else {
-            auto add = [&](auto clear) {
-              uint32_t pf[NB][2];
+            // two: weights in two bf16 parts
+            auto add = [&](auto two, auto clear) {
+              using P = typename std::conditional<decltype(two)::value, __nv_bfloat16, __half>::type;
+              uint32_t pf[NB][2], pl[NB][2];
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) pf[nb][h] = turn8x8(pack2(s[nb][2 * h], s[nb][2 * h + 1], (__half*)nullptr));
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t w = pack2(s[nb][2 * h], s[nb][2 * h + 1], (P*)nullptr);
+                  pf[nb][h] = turn8x8(w);
+                  if constexpr (decltype(two)::value)
+                    pl[nb][h] = turn8x8(pack2(s[nb][2 * h] - __uint_as_float(w << 16),
+                                              s[nb][2 * h + 1] - __uint_as_float(w & 0xffff0000u), (P*)nullptr));
+                }
 #pragma unroll
               for (int k = 0; k < DT; k += 2) {
                 uint32_t b[4];  // units k and k + 1, each keys 0-7 and 8-15
@@ -864,16 +906,22 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                   uint32_t f[4];
                   e4m3_to_half(__byte_perm(b[2 * u], 0, 0x3120), f[0], f[1]);
                   e4m3_to_half(__byte_perm(b[2 * u + 1], 0, 0x3120), f[2], f[3]);
-                  if constexpr (decltype(clear)::value) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[e] &= keep(e >> 1);
+                  for (int e = 0; e < 4; ++e) {
+                    if constexpr (decltype(two)::value) f[e] = half2_to_bf16(f[e]);
+                    if constexpr (decltype(clear)::value) f[e] &= keep(e >> 1);
                   }
 #pragma unroll
-                  for (int nb = 0; nb < NB; ++nb) mma16<false>(o[k + u][nb], f, pf[nb][0], pf[nb][1]);
+                  for (int nb = 0; nb < NB; ++nb) {
+                    mma16<decltype(two)::value>(o[k + u][nb], f, pf[nb][0], pf[nb][1]);
+                    if constexpr (decltype(two)::value) mma16<true>(o[k + u][nb], f, pl[nb][0], pl[nb][1]);
+                  }
                 }
               }
             };
-            if (exact) {
+            if (exact && !beyond) {
+              add(std::true_type(), std::true_type());
+            } else if (exact) {
 #pragma unroll 1
               for (int j = 0; j < min(tail, 16); ++j) {
                 float w[NB][2];  // of key j, rows 2t and 2t + 1
@@ -898,9 +946,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
                 }
               }
             } else if (tail < 16) {
-              add(std::true_type());
+              add(std::false_type(), std::true_type());
             } else {
-              add(std::false_type());
+              add(std::false_type(), std::false_type());
             }
           }
         }

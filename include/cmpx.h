@@ -245,14 +245,15 @@ CMPX_API int cmpx_attention_select_path(int dtype, const void* Q, const void* K,
  * bf16 with head_dim 64 or 128 run tensor-core kernels (a flash-decoding
  * kernel for few query rows per kv head, a tcgen05 kernel for more; softmax
  * weights are rounded to 16 bits once; the flash-decoding kernel rounds them
- * to fp16 over an 8-bit cache, and not at all where value scales lie far apart).  They take pages of 8, 16, 32, ... keys (8-bit caches: 16, 32, ...,
+ * to fp16 over an 8-bit cache, or to 16 bits in fp32's range where value scales
+ * lie far apart).  They take pages of 8, 16, 32, ... keys (8-bit caches: 16, 32, ...,
  * with contiguous scales of a page), 16-byte aligned addresses and strides of
  * 16-byte multiples.  fp32, other head_dim up to 512 and other layouts run a
  * CUDA-core kernel, which is correct but slow.  Keys and values of an 8-bit
  * cache are to every kernel what cmpx_kv_cache_read gives in the queries' type:
- * code * 2^e rounded to it, beyond its largest finite value that value.  (Of
- * bf16's range flash decoding leaves out the ends: parts of a 2^-133 below
- * normal values, and a key that e4m3 rounds up to 2^128 stays that.)
+ * code * 2^e, beyond the type's largest finite value that value.  (Elements
+ * below its normal range may be rounded to it or not, by half a step of fp16's,
+ * 2^-25; a key that e4m3 rounds up to 2^128 stays that in flash decoding.)
  *
  * All strides are in elements.  The element stride within a head is 1. */
 typedef struct {

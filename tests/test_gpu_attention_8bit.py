@@ -10,7 +10,12 @@ result the second part is at most
 
     2^-25 * (max_j w_j * sum_j |v_j|  +  max_j w_j 2^e_j * sum_j |code_j|)
 
-over the visible keys."""
+over the visible keys.
+
+What lies below fp16's normal range may be taken as it is or rounded to fp16,
+so elements of keys and values are off by 2^-25 at most for fp16 queries: a
+score by scale * sum_d |q_d| 2^-25 (a weight by twice that, as in
+seq_reference), the result by 2^-25, another 2^-25 its own rounding there."""
 import contextlib
 import math
 
@@ -79,7 +84,7 @@ class Cache:
         scale = 1 / math.sqrt(d) if scale is None else scale
         kk, vv = (read_as(c, b, q.dtype) for c, b in (self.k, self.v))
         want, tol = attend(q, kk, vv, scale, True, u_w, U[q.dtype])
-        step = 2.0**-25 if q.dtype == F16 else 2.0**-134  # half of the output's smallest
+        step = 2 * 2.0**-25 if q.dtype == F16 else 2.0**-134  # half of the output's smallest; the values'
         for i in range(n):
             lim = max(0, min(length, length - n + i + 1))
             if lim == 0:
@@ -90,6 +95,9 @@ class Cache:
             e = torch.where(self.v[1][:lim].repeat_interleave(hq // hkv, 1).t() == 255, 0.0, e)
             codes = self.v[0][:lim].double().nan_to_num().abs().sum(0).repeat_interleave(hq // hkv, 0)
             vals = vv[:lim].nan_to_num().abs().sum(0).repeat_interleave(hq // hkv, 0)
+            if q.dtype == F16:
+                spread = torch.einsum("hj,jhd->hd", w, vv[:lim].repeat_interleave(hq // hkv, 1).abs().nan_to_num())
+                tol[i] += 2 * abs(scale) * 2.0**-25 * q[i].double().abs().sum(-1, keepdim=True) * spread
             tol[i] += step + 2.0**-25 * (w.amax(-1, keepdim=True) * vals + (w * e).amax(-1, keepdim=True) * codes)
         check(got, want, tol, what)
 
@@ -266,3 +274,64 @@ def test_the_largest_value(cuda, dtype, path):
     read = cx.kv_cache_read(kc, vc, torch.tensor([19], device="cuda"), ks, vs, dtype=dtype)[1]
     assert torch.equal(read, v)
     assert torch.equal(out, v.repeat_interleave(2, 1))
+
+
+SPREAD = {  # scale bytes of a sequence's values: 14 and 28 binades at random, a weighty first token of small values, ...
+    "spread": lambda x: torch.randint(112, 126, (x,), generator=torch.Generator().manual_seed(1)),
+    "wide": lambda x: torch.randint(100, 128, (x,), generator=torch.Generator().manual_seed(2)),
+    "sink": lambda x: torch.where(torch.arange(x) == 0, 105, 120),
+    "steps": lambda x: 100 + torch.arange(x) // 16 % 20,
+    "zeros": lambda x: torch.where(torch.arange(x) % 64 == 5, 127, 111),
+}
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [1, 5, 24])
+@pytest.mark.parametrize("scales", list(SPREAD))
+def test_value_scales_that_vary(cuda, scales, n, dtype, path):
+    """The reference of the weights follows the strips up and down: no bits are lost."""
+    length = 900
+    v = scaled(length, 2, 128, SPREAD[scales](length), 15)
+    if scales == "zeros":
+        v[0][torch.arange(length) % 64 == 5] = 0
+    k = normal(length, 2, 128, 14)
+    c = Cache(k, v)
+    q = queries(n, 4, 128, dtype)
+    if scales == "sink":  # queries that look at the first key
+        q += read_as(k[0][:1], k[1][:1], dtype)[0].repeat_interleave(2, 0).to(dtype)
+    with forced(path):
+        out = c.run(q)
+        for _ in range(2):
+            assert torch.equal(c.run(q), out)
+    finish()
+    c.check(out, q, scales, U[dtype])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_strips_out_of_the_band_stay_matrix_products(cuda, dtype):
+    """Measured 1.5 times as long; key by key it was five times."""
+
+    def best(high):
+        g = gen(16)
+        kc, vc = (torch.randint(0, 120, (600, 8, 64, 128), generator=g, dtype=torch.uint8, device="cuda").view(E4M3)
+                  for _ in range(2))
+        ks = torch.full((600, 8, 64), 120, dtype=torch.uint8, device="cuda").view(E8M0)
+        vs = torch.randint(112, high, (600, 8, 64), generator=g, dtype=torch.uint8, device="cuda").view(E8M0)
+        table = torch.randperm(600, generator=g, device="cuda").int().view(12, 50)
+        lens = torch.full((12,), 3200, dtype=torch.int32, device="cuda")
+        q = queries(12, 32, 128, dtype)
+        times = []
+        for _ in range(7):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(5):
+                cx.attention_paged(q, kc, vc, table, lens, key_scale=ks, value_scale=vs)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) / 5)
+        return min(times)
+
+    even, varied = best(114), best(126)
+    print(f"{dtype}: {even * 1e3:.1f} us, scales of 14 binades {varied * 1e3:.1f}")
+    assert varied <= 2.5 * even
