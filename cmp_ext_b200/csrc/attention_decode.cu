@@ -569,18 +569,18 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
               qf[k][nb][1] = x.y;
             }
             if constexpr (FMT == 1) {
-              uint32_t top = 0;  // largest magnitude, as bf16 bits
+              uint32_t top = 0;  // largest finite magnitude, as bf16 bits
 #pragma unroll
               for (int k = 0; k < DT; ++k)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  top = max(top, max(qf[k][nb][e] & 0x7fffu, qf[k][nb][e] >> 16 & 0x7fffu));
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t a0 = qf[k][nb][e] & 0x7fffu, a1 = qf[k][nb][e] >> 16 & 0x7fffu;
+                  top = max(top, max(a0 < 0x7f80u ? a0 : 0u, a1 < 0x7f80u ? a1 : 0u));
+                }
               top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
               top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
               // the row times 2^(14 - k), 2^k <= top < 2^(k + 1): below 2^15
-              const int e2 = int(top >> 7);
-              const bool plain = e2 == 0 || e2 == 255;
-              const float down = plain ? 1.0f : __uint_as_float(uint32_t(min(268 - e2, 254)) << 23);
+              const float down = __uint_as_float(min(268u - (top >> 7), 254u) << 23);
               up = 1.0f / down;
 #pragma unroll
               for (int k = 0; k < DT; ++k)

@@ -335,3 +335,30 @@ def test_strips_out_of_the_band_stay_matrix_products(cuda, dtype):
     even, varied = best(114), best(126)
     print(f"{dtype}: {even * 1e3:.1f} us, scales of 14 binades {varied * 1e3:.1f}")
     assert varied <= 2.5 * even
+
+
+@pytest.mark.parametrize("path", KERNELS)
+@pytest.mark.parametrize("n", [1, 9])
+def test_queries_with_an_infinity(cuda, n, path):
+    """Scores of -inf hide a key, whatever the row's other elements are (in
+    fp16, which flash decoding multiplies, 1e5 would be an infinity too)."""
+    length = 60
+    codes, byte = normal(length, 2, 64, 17)
+    codes[:, :, 0] = torch.where(torch.arange(length) % 3 == 0, -1.0, 1.0).to(codes).view(-1, 1)  # q[0] hides two of three
+    codes[:, :, 1] = 1
+    c = Cache((codes, byte), normal(length, 2, 64, 18))
+    q = queries(n, 4, 64, BF16)
+    q[:, :2, 0] = -math.inf
+    q[:, :2, 1] = 1e5
+    q[:, 2:, :2] = torch.tensor([1e5, -1e5])  # no infinity: as ever
+    with forced(path):
+        out = c.run(q)
+    finish()
+    assert out[:, :2].isnan().all()  # one of three scores is +inf
+    assert out[:, 2:].isfinite().all()
+    c.k[0][:, :, 0] = 1
+    c = Cache(c.k, c.v)
+    with forced(path):
+        out = c.run(q)
+    finish()
+    assert not out[:, :2].any()  # all are -inf: zeros
