@@ -17,8 +17,8 @@
 // sixteen would, and a warp's state (D x 8 sums) leaves registers for sixteen
 // warps an SM, which is what hides the latency of the strip's chain of
 // dependent steps.  48 single tokens of 32 / 8 heads of 128 over 1000 to 24000
-// keys in an e4m3 cache: 440 us with rows along the 16-wide side, 122 us now
-// (5.7 TB/s of what it has to read, 88% of the copy rate).
+// keys in an e4m3 cache: 122-130 us (5.4-5.7 TB/s of what it has to read, 82-88%
+// of the copy rate), 454 with rows along the 16-wide side.
 //
 // Work: units (sequence, kv head, ROWS rows) of tiles (64 or 128 keys) in one
 // list, each unit's beginning and end weighted like two tiles; block c of P
@@ -1154,8 +1154,10 @@ int decode_keys(const SeqProblem& p, bool q8) {
                    : (q8 ? DecodeCfg<128, true, 1>::KEYS : DecodeCfg<128, false, 1>::KEYS);
 }
 int64_t decode_blocks(const DeviceInfo& dev, int rows) { return int64_t(dev.num_sms) * (rows == 8 ? 2 : 1); }
-// Sequences that cannot be long: splitting them among blocks would save less
-// than the second kernel costs.
+// Sequences that cannot be long: splitting them among blocks saves less than
+// the second kernel costs.  Whole and split, 32 / 8 heads of 128, one token over
+// 512 keys 11.1 and 14.3 us, over 1024 15.6 and 14.7; 16 tokens 12.7 and 16.2,
+// 18.2 and 18.5; 128 tokens, which need no splitting, 62 and 54, 97 and 93.
 bool decode_whole(const SeqProblem& p) { return (p.table != nullptr ? p.max_keys : p.tokens_kv) <= 512; }
 
 // More places than any lengths can make of the problem (64 keys, 8 rows each).

@@ -124,8 +124,6 @@ cudaError_t launch_simt_typed(const SeqProblem& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-int64_t max64(int64_t a, int64_t b) { return a > b ? a : b; }
-
 // Checks everything the host can see.  CMPX_OK with *empty set: nothing to do.
 int validate_seq(const cmpx_attention_seq_args* a, bool* empty) {
   *empty = false;
@@ -220,8 +218,10 @@ int64_t typical_rows(const cmpx_attention_seq_args* a, const SeqProblem& p) {
 
 // The kernel that runs a checked, non-empty problem, or -1.  Few query rows a
 // kv head run the flash-decoding kernel, whose units hold at most 16 of them;
-// more the tcgen05 kernel (48 single tokens, 4 rows a kv head, over an e4m3
-// cache: 122 against 1940 us when it had one kernel for all).
+// more the tcgen05 kernel.  16 sequences over 4000 keys, 32 / 8 heads of 128,
+// flash decoding against tcgen05: 4 rows 53 and 76 us (e4m3 cache 39 and 89),
+// 16 rows 57 and 77 (52 and 90), 24 rows, where keys are read twice, 95 and 77
+// (82 and 90); 64 sequences over 1000 keys, 24 rows: 113 and 83 (121 and 98).
 int seq_path(const cmpx_attention_seq_args* a, const SeqProblem& p) {
   const bool simt_ok = a->head_dim <= kSimtMaxD && (a->tokens_q * a->heads_q + 3) / 4 <= INT_MAX;
   const bool tile_ok = seq_tile_ok(p, a->dtype, a->kv_dtype);

@@ -143,8 +143,8 @@ __device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int
     for (int i = 0; i < NV; ++i) acc[i] = fmaf(w, load(vr + lane + 32 * i, vs), acc[i]);
   }
 }
-// First token that no sequence holds any more (cu_seqlens_q[batch], clamped),
-// and the number of tokens before the first sequence.
+// x: tokens before the first sequence; y: first token behind the last one
+// (the first and last offset, clamped).
 __device__ __forceinline__ int2 seq_rest(const SeqProblem& p) {
   if (p.cu_q == nullptr) return make_int2(0, p.batch * p.uniform_n);
   return make_int2(min(max(__ldg(p.cu_q), 0), p.tokens_q), min(max(__ldg(p.cu_q + p.batch), 0), p.tokens_q));

@@ -15,14 +15,14 @@
 // D = 128) and O += P V (512), and 128 threads, one a row, turn S into P:
 // 16384 exponentials at 16 a cycle are 1024 cycles.  Two tiles in turn keep
 // both units busy.  Measured: 4300 cycles a key block of both tiles (2048
-// would be the units' own time), 577 us and 920 TFLOP/s on two prompts of 8192
-// tokens, 16 / 4 heads of 128, at clocks that the power limit holds near
-// 1.6 GHz; what is left is each tile's chain of softmax (1800 cycles), P V,
-// its completion and the next Q K^T (1500).  S is read into registers and P written over it in tensor
-// memory, from where the P V product takes it as its A operand: P crosses
-// neither shared memory, whose bandwidth the two products' operands need
-// (the same product from shared memory would read 64 KB a block and tile
-// instead of 32), nor a proxy fence.
+// would be the units' own time), 566-583 us and 910-937 TFLOP/s on two prompts
+// of 8192 tokens, 16 / 4 heads of 128, at clocks that the power limit holds
+// near 1.6 GHz; what is left is each tile's chain of softmax (1800 cycles),
+// P V, its completion and the next Q K^T (1500).  S is read into registers and
+// P written over it in tensor memory, from where the P V product takes it as
+// its A operand: P crosses neither shared memory, whose bandwidth the two
+// products' operands need (the same product from shared memory would read 64 KB
+// a block and tile instead of 32), nor a proxy fence.
 //
 // Running maximum: O is rescaled only when a row's maximum grew by more than
 // 2^8 over the one its weights are taken against (fp32 sums and 16-bit
@@ -852,9 +852,12 @@ int64_t tile_count(const SeqProblem& p) {
 // 2.2 us a key block takes: the longest walk of a block, and all walks over the
 // SMs.  A block's beginning, end and partial result cost as much as five key
 // blocks, the joining kernel two.  Lengths are on the device: the longest walk
-// is taken to be as long as a sequence can be, a typical one 0.6 of it.  (16
-// sequences of 713 new tokens over 200 to 6000 keys: 142 us unsplit, 110
-// split in two.)
+// is taken to be as long as a sequence can be, a typical one 0.6 of it.
+// 32 / 8 heads of 128, unsplit and by this rule: 64 new tokens over 16000 keys
+// 253 and 54 us, over 2000 39 and 20 (24 with a page table for 131072 keys), 8 x
+// 100 over 800 to 8000 keys 138 and 132, 16 x 100 over 6000 205 and 205; where
+// all sequences are as long as the longest, it splits too much: 4 x 200 over
+// 4000 73 and 93.
 int tile_splits(const SeqProblem& p, const DeviceInfo& dev) {
   const double blocks = double(tile_count(p)) * p.heads_kv, sms = dev.num_sms;
   const double keys = ((p.table != nullptr ? p.max_keys : p.tokens_kv) + 127) / 128;

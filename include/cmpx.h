@@ -241,7 +241,9 @@ CMPX_API int cmpx_attention_select_path(int dtype, const void* Q, const void* K,
  *   no query of a sequence sees never change its rows, NaN and infinities
  *   among them.
  *
- * Softmax statistics and sums are fp32; the output is rounded once.  fp16 /
+ * Softmax statistics and sums are fp32; the output is rounded once.  Sums of
+ * weights (2^8 at most) times values come before the division, so values whose
+ * magnitude times the number of keys passes 2^120 may overflow.  fp16 /
  * bf16 with head_dim 64 or 128 run tensor-core kernels (a flash-decoding
  * kernel for few query rows per kv head, a tcgen05 kernel for more; softmax
  * weights are rounded to 16 bits once; the flash-decoding kernel rounds them
