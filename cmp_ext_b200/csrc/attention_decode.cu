@@ -1052,11 +1052,16 @@ __global__ void __launch_bounds__(DecodeCfg<D, Q8, NB>::THREADS, DecodeCfg<D, Q8
             a.joints[int64_t(info.q0 + row.token) * p.heads_q + row.head] =
                 int(blockIdx.x) | info.pieces << 12 | r << 24;
           if (__any_sync(0xffffffffu, bad) && tot[y].y > 0.0f && tot[y].y <= 3.4028234663852886e38f &&
-              seq_hidden_bad<typename std::conditional<Q8, uint8_t, T>::type, D>(
-                  p, info.b, info.k0, info.hk, max(row.lim, info.piece_key), min(info.len, info.key + KEYS))) {
-            const T* q = static_cast<const T*>(p.Q) + int64_t(info.q0 + row.token) * p.q_token + row.head * p.q_head;
-            redo_row<T, D, Q8>(p, info.b, info.k0, info.hk, q, info.piece_key, min(row.lim, info.key + KEYS), tot[y].x,
-                               acc[y]);
+              seq_last_bad<T, D, Q8>(p, info.b, info.k0, info.hk, max(row.lim, info.piece_key),
+                                     min(info.len, info.key + KEYS)) >= 0) {
+            const T* const q[1] = {static_cast<const T*>(p.Q) + int64_t(info.q0 + row.token) * p.q_token +
+                                   row.head * p.q_head};
+            const int lims[1] = {min(row.lim, info.key + KEYS)};
+            const float at[1] = {tot[y].x};
+            float sums[1][D / 32];
+            redo_rows<T, D, Q8, 1>(p, info.b, info.k0, info.hk, q, info.piece_key, lims, at, sums);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) acc[y][c] = sums[0][c];
           }
           if (flags & kWhole) {
             const float inv = tot[y].y == 0.0f ? 0.0f : 1.0f / tot[y].y;

@@ -74,73 +74,134 @@ __device__ __forceinline__ void rec_err(int* err, volatile int* abort, int code)
   *abort = 1;
   atomicCAS(err, 0, code);
 }
-// Whether a value of keys [from, to) of a sequence is not finite (a warp
-// looks; T the values' type, or uint8_t for e4m3 codes).  A row whose result
-// is not finite although its sum is has to be computed again only if such a
-// value is among those it may not see: it reaches the row through 0 * NaN.
-template <typename T, int D>
-__device__ __forceinline__ bool seq_hidden_bad(const SeqProblem& p, int b, int k0, int hk, int from, int to) {
-  const int lane = threadIdx.x & 31;
-  bool bad = false;
-  for (int j = from; j < to; ++j) {
-    int64_t at = int64_t(k0 + j) * p.v.row;
-    if (p.table != nullptr) {
-      const int page = __ldg(p.table + b * p.table_stride + j / p.page_size), slot = j % p.page_size;
-      if (page < 0 || page >= p.pages) continue;  // zeros
-      at = page * p.v.page + slot * p.v.row;
-      if (sizeof(T) == 1) bad = bad || p.v.scale[page * p.v.s_page + hk * p.v.s_head + slot * p.v.s_row] == 255;
-    }
-    const T* v = static_cast<const T*>(p.v.base) + at + hk * p.v.head;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      if constexpr (sizeof(T) == 1) {
-        bad = bad || (v[lane + 32 * i] & 0x7f) == 0x7f;
-      } else {
-        const float x = float(v[lane + 32 * i]);
-        bad = bad || x - x != 0.0f;
-      }
-    }
+// Place of key j of a sequence's kv head hk in K and V (elements), and its
+// scales of an 8-bit cache; false for a page that is none (zeros).
+struct SeqKey {
+  int64_t k, v;
+  uint32_t k_scale, v_scale;
+};
+template <bool Q8>
+__device__ __forceinline__ bool seq_key(const SeqProblem& p, int b, int k0, int hk, int j, SeqKey& x) {
+  if (p.table == nullptr) {
+    x.k = int64_t(k0 + j) * p.k.row + hk * p.k.head;
+    x.v = int64_t(k0 + j) * p.v.row + hk * p.v.head;
+    return true;
   }
-  return __any_sync(0xffffffffu, bad);
+  const int page = __ldg(p.table + b * p.table_stride + j / p.page_size), slot = j % p.page_size;
+  if (page < 0 || page >= p.pages) return false;
+  x.k = page * p.k.page + slot * p.k.row + hk * p.k.head;
+  x.v = page * p.v.page + slot * p.v.row + hk * p.v.head;
+  if constexpr (Q8) {
+    x.k_scale = p.k.scale[page * p.k.s_page + hk * p.k.s_head + slot * p.k.s_row];
+    x.v_scale = p.v.scale[page * p.v.s_page + hk * p.v.s_head + slot * p.v.s_row];
+  }
+  return true;
 }
-// One row over keys [kbeg, kend) of a sequence from its definition: the sums
-// of weights 2^(x - m) times values.  A warp computes it, lane i the columns
-// i, i + 32, ...
+// The last of keys [from, to) of a sequence whose value is not finite, or -1
+// (a warp looks, a lane a key).  A row whose result is not finite although its
+// sum is has to be computed again only if such a value is among those it may
+// not see: it reaches the row through 0 * NaN.  Rows of 16 bytes, as the
+// tensor-core kernels take them.
 template <typename T, int D, bool Q8>
-__device__ __forceinline__ void redo_row(const SeqProblem& p, int b, int k0, int hk, const T* q, int kbeg, int kend,
-                                         float m, float (&acc)[D / 32]) {
-  const int lane = threadIdx.x & 31;
-  constexpr int NV = D / 32;
-  using KV = typename std::conditional<Q8, uint8_t, T>::type;
-  auto load = [](const KV* at, float up) -> float {
-    if constexpr (Q8) return held<T>(*at, up);
-    else return ldf(at);
-  };
+__device__ __forceinline__ int seq_last_bad(const SeqProblem& p, int b, int k0, int hk, int from, int to) {
+  int last = -1;
+  for (int j = from + int(threadIdx.x & 31); j < to; j += 32) {
+    SeqKey x;
+    if (!seq_key<Q8>(p, b, k0, hk, j, x)) continue;
+    const uint4* row = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.v.base) + x.v * (Q8 ? 1 : 2));
+    bool bad = Q8 && x.v_scale == 255;
+#pragma unroll 2
+    for (int i = 0; i < D * (Q8 ? 1 : 2) / 16; ++i) {
+      const uint4 u = __ldg(row + i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
-  for (int j = kbeg; j < kend; ++j) {
-    int64_t ko = int64_t(k0 + j) * p.k.row, vo = int64_t(k0 + j) * p.v.row;
-    float ks = 1.0f, vs = 1.0f;
-    if (p.table != nullptr) {
-      const int page = __ldg(p.table + b * p.table_stride + j / p.page_size), slot = j % p.page_size;
-      if (page < 0 || page >= p.pages) continue;  // reads as zeros: nothing to add
-      ko = page * p.k.page + slot * p.k.row;
-      vo = page * p.v.page + slot * p.v.row;
-      if (Q8) {
-        ks = e8m0_to_float(p.k.scale[page * p.k.s_page + hk * p.k.s_head + slot * p.k.s_row]);
-        vs = e8m0_to_float(p.v.scale[page * p.v.s_page + hk * p.v.s_head + slot * p.v.s_row]);
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (Q8) {
+          bad = bad || __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
+        } else {
+          constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+          bad = bad || (w[k] & E) == E || (w[k] >> 16 & E) == E;
+        }
       }
     }
-    const KV* kr = static_cast<const KV*>(p.k.base) + ko + hk * p.k.head;
-    const KV* vr = static_cast<const KV*>(p.v.base) + vo + hk * p.v.head;
-    float dot = 0.0f;
+    if (bad) last = j;
+  }
+  return __reduce_max_sync(0xffffffffu, last);
+}
+// R rows of a kv head from their definition, row r over keys [kbeg, lim[r]) of
+// a sequence: the sums of weights 2^(x - m[r]) times values.  A warp computes
+// them, lane i the columns i, i + 32, ... of the sums.  32 keys at a time, a
+// lane a key's scores and then all lanes a key's value: key by key and row by
+// row, with a sum over the lanes for each score, a key took a microsecond (40 x
+// 40 new tokens over 16384 keys with a NaN beside them 260 ms, this way 60, and
+// 0.8 without one), and a million of them the time that other warps wait for.
+template <typename T, int D, bool Q8, int R>
+__device__ __forceinline__ void redo_rows(const SeqProblem& p, int b, int k0, int hk, const T* const (&q)[R], int kbeg,
+                                          const int (&lim)[R], const float (&m)[R], float (&acc)[R][D / 32]) {
+  const int lane = threadIdx.x & 31;
+  constexpr int NV = D / 32, CHUNK = 8;  // of columns
+  int kend = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) dot = fmaf(ldf(q + lane + 32 * i), load(kr + lane + 32 * i, ks), dot);
+  for (int r = 0; r < R; ++r) {
+    kend = max(kend, lim[r]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float w = ex2_approx(fmaf(dot, p.scale_log2, -m));
+    for (int i = 0; i < NV; ++i) acc[r][i] = 0.0f;
+  }
+#pragma unroll 1
+  for (int base = kbeg; base < kend; base += 32) {
+    SeqKey x = {};  // (of a page that is none, or behind the last key: the first row, not used)
+    const bool there = base + lane < kend && seq_key<Q8>(p, b, k0, hk, base + lane, x);
+    if (!there) x = SeqKey{};
+    float w[R];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] = fmaf(w, load(vr + lane + 32 * i, vs), acc[i]);
+    for (int r = 0; r < R; ++r) w[r] = 0.0f;
+    const float up = Q8 ? e8m0_to_float(x.k_scale) : 1.0f;
+#pragma unroll(R == 1 ? 1 : 2)
+    for (int c = 0; c < D; c += CHUNK) {
+      float k[CHUNK];
+      if constexpr (Q8) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.k.base) + x.k + c));
+#pragma unroll
+        for (int i = 0; i < CHUNK; i += 2) {
+          const uint32_t two = dequant2((i < 4 ? u.x : u.y) >> 8 * (i & 3) & 0xffffu, up, (T*)nullptr);
+          k[i] = ldf(reinterpret_cast<const T*>(&two));
+          k[i + 1] = ldf(reinterpret_cast<const T*>(&two) + 1);
+        }
+      } else {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.k.base) + x.k + c));
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) k[i] = ldf(reinterpret_cast<const T*>(&u) + i);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(q[r] + c));
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) w[r] = fmaf(ldf(reinterpret_cast<const T*>(&u) + i), k[i], w[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) w[r] = ex2_approx(fmaf(w[r], p.scale_log2, -m[r]));
+    const float vs = Q8 ? e8m0_to_float(x.v_scale) : 1.0f;
+    const unsigned present = __ballot_sync(0xffffffffu, there);
+#pragma unroll(R == 1 ? 4 : 2)
+    for (int t = 0; t < 32; ++t) {
+      const float st = Q8 ? __shfl_sync(0xffffffffu, vs, t) : 1.0f;
+      const int64_t at = __shfl_sync(0xffffffffu, (long long)x.v, t);
+      const bool on = present >> t & 1;
+      float v[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (Q8) v[i] = held<T>(static_cast<const uint8_t*>(p.v.base)[at + lane + 32 * i], st);
+        else v[i] = ldf(static_cast<const T*>(p.v.base) + at + lane + 32 * i);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float wt = __shfl_sync(0xffffffffu, w[r], t);
+        if (on && base + t < lim[r])
+#pragma unroll
+          for (int i = 0; i < NV; ++i) acc[r][i] = fmaf(wt, v[i], acc[r][i]);
+      }
+    }
   }
 }
 // x: tokens before the first sequence; y: first token behind the last one

@@ -714,27 +714,42 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::THREADS, 1)
       // not finite although the weights are: a value the row may not see (see above)
       bad = bad && valid && l > 0.0f && l <= 3.4028234663852886e38f;
       unsigned again = __ballot_sync(0xffffffffu, bad);
+      int last_bad = -1;  // of the keys that one of them may not see
+      if (again != 0)
+        last_bad = seq_last_bad<T, D, Q8>(p, seq, s.k0, hk, max(__reduce_min_sync(0xffffffffu, bad ? lim : kend), jb * 128),
+                                          min(kend, (jb + nt) * 128));
+      again = __ballot_sync(0xffffffffu, bad && last_bad >= lim);
       while (again != 0) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        const int tok = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
-        const int kl = min(__shfl_sync(0xffffffffu, lim, src), kend);
-        if (!seq_hidden_bad<typename std::conditional<Q8, uint8_t, T>::type, D>(p, seq, s.k0, hk, max(kl, jb * 128),
-                                                                               min(kend, (jb + nt) * 128)))
-          continue;
-        const float mm = __shfl_sync(0xffffffffu, m, src), ii = __shfl_sync(0xffffffffu, inv, src);
-        const T* q = static_cast<const T*>(p.Q) + (s.q0 + tok) * p.q_token + hd * p.q_head;
-        T* of = static_cast<T*>(p.O) + (s.q0 + tok) * p.o_token + hd * p.o_head;
-        float* pf = a.splits > 1 ? a.part_o + (int64_t(blockIdx.z) * p.tokens_q * p.heads_q +
-                                               int64_t(s.q0 + tok) * p.heads_q + hd) * D
-                                 : nullptr;
-        float acc[D / 32];
-        redo_row<T, D, Q8>(p, seq, s.k0, hk, q, jb * 128, kl, mm, acc);
-        __syncwarp();  // behind the stores of the row's own thread, which these replace
+        constexpr int R = 2;  // rows that share a walk over their keys (of 4 and 8 all calls' loops were 2% slower)
+        const T* q[R];
+        int lims[R], from[R];
+        float at[R], sums[R][D / 32];
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          if (a.splits > 1) pf[lane + 32 * i] = acc[i];
-          else stf(of + lane + 32 * i, acc[i] * ii);
+        for (int r = 0; r < R; ++r) {
+          from[r] = again != 0 ? __ffs(again) - 1 : -1;
+          again &= again - 1;
+          const int src = max(from[r], 0);
+          const int tok = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
+          const int sees = min(__shfl_sync(0xffffffffu, lim, src), kend);
+          lims[r] = from[r] < 0 ? 0 : sees;
+          at[r] = __shfl_sync(0xffffffffu, m, src);
+          q[r] = static_cast<const T*>(p.Q) + (from[r] < 0 ? 0 : (s.q0 + tok) * p.q_token + hd * p.q_head);
+        }
+        redo_rows<T, D, Q8, R>(p, seq, s.k0, hk, q, jb * 128, lims, at, sums);
+        __syncwarp();  // behind the stores of the rows' own threads, which these replace
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int src = max(from[r], 0);
+          const int tok = __shfl_sync(0xffffffffu, token, src), hd = __shfl_sync(0xffffffffu, head, src);
+          const float ii = __shfl_sync(0xffffffffu, inv, src);
+          if (from[r] < 0) continue;
+          T* of = static_cast<T*>(p.O) + (s.q0 + tok) * p.o_token + hd * p.o_head;
+          float* pf = a.part_o + (int64_t(blockIdx.z) * p.tokens_q * p.heads_q + int64_t(s.q0 + tok) * p.heads_q + hd) * D;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            if (a.splits > 1) pf[lane + 32 * i] = sums[r][i];
+            else stf(of + lane + 32 * i, sums[r][i] * ii);
+          }
         }
       }
     }
