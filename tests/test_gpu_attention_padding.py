@@ -99,3 +99,30 @@ def test_offsets_that_do_not_ascend(cuda, batch, width, path):
     for i, n in enumerate((100, 5, 128)):
         want, tol = attend(q[i : i + 1], keys[0][:n], keys[1][:n], 1 / math.sqrt(d), True, U[F16], U[F16])
         check(out[i : i + 1], want, tol, f"row {i}")
+
+
+@pytest.mark.parametrize("path", ["tc", "skinny", "simt"])
+def test_a_captured_padded_batch(cuda, path):
+    """One graph, replayed with other lengths: rows that a longer batch wrote are zeros again in a shorter one."""
+    total = 700
+    q, k, v = qkv(total, 8, 2, 64, BF16, 3)
+    at = cu(0, 300, 650)
+    cx._set_path(path)
+    try:
+        cx.attention_varlen(q, k, v, at)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = cx.attention_varlen(q, k, v, at)
+        for offsets in ((0, 300, 650), (0, 10, 11), (200, 200, 700), (0, 0, 0), (50, 400, 401), (0, 699, 700)):
+            at.copy_(torch.tensor(offsets, dtype=torch.int32))
+            g.replay()
+            torch.cuda.synchronize()
+            assert cabi.device_error() == 0
+            assert torch.equal(out, cx.attention_varlen(q, k, v, at))
+            assert not out[: offsets[0]].any() and not out[offsets[2] :].any()
+            for a, b in zip(offsets, offsets[1:]):
+                n = min(b - a, 20)
+                want, tol = attend(q[a : a + n], k[a : a + n], v[a : a + n], 1 / 8, True, U[BF16], U[BF16])
+                check(out[a : a + n], want, tol, f"{offsets}")
+    finally:
+        cx._set_path("auto")
